@@ -8,6 +8,7 @@ transformed scale tensors only; all compute runs in the library's CUDA kernels.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os as _os
 import threading
@@ -1063,6 +1064,89 @@ def k_grouped_bf16_gemm_tn_contiguous(a, b, d, ks_cpu, grouped_layout, c=None, c
                       accumulate=c is not None, layout=grouped_layout, use_psum_layout=use_psum_layout, stochastic=_stochastic(epilogue, c, d))
     args.lda, args.ldb, args.ldd = m, n, n
     check(lib.dg_k_grouped_fp8_gemm_contiguous(C.byref(args)))
+
+
+# ------------------------------------------------------------------------------------------------
+# BF16 activations with packed E2M1 weights (no counterpart in the reference, whose FP4 GEMMs quantise the activations)
+# ------------------------------------------------------------------------------------------------
+def _bf16_fp4_args(a, b, d, n, k, groups, recipe_b, **kw) -> GemmArgs:
+    (w, sf), (gran_mn, gran_k) = b, tuple(recipe_b)
+    _require(a.dtype == torch.bfloat16 and w.dtype == kPackedFP4, "a: bfloat16, b: packed FP4 (int8)")
+    _require(a.stride(-1) == 1 and w.stride(-1) == 1, "major_a == cute::UMMA::Major::K and major_b == cute::UMMA::Major::K")
+    _require(all(t.is_cuda and t.device == d.device for t in (a, w, sf, d)), "a, b, d are CUDA tensors of one device")
+    _check_cd(d)
+    m = a.size(0)
+    sf = transform_sf_into_required_layout(sf, n, k, (gran_mn, gran_k), groups if w.dim() == 3 else None)
+    args = GemmArgs()
+    args.a, args.b, args.sfb, args.d = a.data_ptr(), w.data_ptr(), sf.data_ptr(), d.data_ptr()
+    args.m, args.n, args.k, args.num_groups = m, n, k, groups
+    args.a_dtype, args.b_dtype, args.d_dtype = _lib.DG_BF16, _lib.DG_FP4_E2M1_X2, _d_dtype(d)
+    args.major_a = args.major_b = _lib.DG_MAJOR_K
+    # (the pitch of a single row says nothing: torch may report any stride for it)
+    args.lda, args.ldb, args.ldd = (a.stride(0), w.stride(-2), d.stride(0)) if m > 1 else (k, w.stride(-2), align(n, 8))
+    args.sfb_pitch, args.gran_k_b = sf.stride(-1), gran_k
+    alpha = kw.get("alpha")
+    args.accumulate, args.has_alpha, args.alpha = int(kw.get("accumulate", False)), int(alpha is not None), 1.0 if alpha is None else float(alpha)
+    layout = kw.get("layout")
+    args.grouped_layout = layout.data_ptr() if layout is not None else None
+    args.stream = _stream()
+    args._keep = sf                  # the scales may be a tensor of this call's own
+    return args
+
+
+def _on_device_of(t: torch.Tensor):
+    """The calls below launch on the device their tensors live on, whichever device is current."""
+    return torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def bf16_fp4_gemm_nt(a, b, d, c=None, recipe_b=(1, 32), compiled_dims: str = "nk", alpha: Optional[float] = None) -> None:
+    """D[M,N] = C + alpha * A[M,K] @ W[N,K]^T for BF16 A and b = (packed E2M1 weights int8 [N, K/2], their scales): the
+    weights an FP8 x FP4 GEMM takes, in the same storage, multiplied with activations that are not quantised.  recipe_b =
+    (1, 32) or (1, 128); scales packed (int32) or FP32 (packed on the fly); D BF16 or FP32; K % 128 == 0.  Any number of
+    rows from a single token on; sums in FP32, one rounding per element (two where C is added to a BF16 D)."""
+    w, _ = b
+    _require(a.dim() == 2 and w.dim() == 2 and d.dim() == 2, "t.dim() == N")
+    (m, k), n = a.shape, w.size(0)
+    _require(m == d.size(0) and n == d.size(1) and k == 2 * w.size(1), "m == m_ and n == n_ and k == k_")
+    _require(d.dtype in (torch.bfloat16, torch.float), "d.scalar_type() == torch::kBFloat16 or d.scalar_type() == torch::kFloat")
+    if c is not None:
+        _check_cd(c)
+        _require(d.dtype == c.dtype and c.shape == d.shape, "d.scalar_type() == c.value().scalar_type()")
+    is_cd_same = c is not None and c.data_ptr() == d.data_ptr()
+    if is_cd_same:
+        _require(c.stride() == d.stride(), "c->sizes() == d.sizes() and c->strides() == d.strides()")
+    if m == 0 or n == 0:
+        return
+    if k == 0:
+        if not is_cd_same:
+            d.copy_(c) if c is not None else d.zero_()
+        return
+    with _on_device_of(d):
+        args = _bf16_fp4_args(a, b, d, n, k, 1, recipe_b, accumulate=c is not None, alpha=alpha)
+        if c is not None and not is_cd_same:
+            d.copy_(c)
+        check(lib.dg_bf16_fp4_gemm(C.byref(args)))
+
+
+def m_grouped_bf16_fp4_gemm_nt_ragged(a, b, d, group_ends, recipe_b=(1, 32), compiled_dims: str = "nk") -> None:
+    """D[r] = A[r] @ W[g(r)]^T for BF16 A [rows, K] sorted by expert and b = (packed E2M1 weights int8 [G, N, K/2], their
+    scales): the expert layer of the 4-bit weights above.  group_ends (int32 [G], on the device, not decreasing) holds the
+    row where each group ends; the groups follow one another without padding or alignment, empty ones included, and rows
+    at or behind group_ends[-1] keep what D holds.  Capturable: a replay follows the ends of that moment.  D BF16."""
+    w, _ = b
+    _require(a.dim() == 2 and w.dim() == 3 and d.dim() == 2, "t.dim() == N")
+    (m, k), (groups, n, _) = a.shape, w.shape
+    _require(m == d.size(0) and n == d.size(1) and k == 2 * w.size(2), "m == m_ and n == n_ and k == k_")
+    _require(n > 0 and k > 0 and groups > 0, "n > 0 and k > 0 and num_groups > 0")
+    _require(w.stride(0) == n * w.stride(1), "the groups of b follow one another")
+    _require(d.dtype == torch.bfloat16, "d.scalar_type() == torch::kBFloat16")
+    _require(group_ends.is_cuda and group_ends.device == d.device and group_ends.dtype == torch.int and group_ends.dim() == 1 and
+             group_ends.is_contiguous() and group_ends.size(0) == groups, "group_ends: contiguous int32 [num_groups] on the device of d")
+    if m == 0:
+        return
+    with _on_device_of(d):
+        args = _bf16_fp4_args(a, b, d, n, k, groups, recipe_b, layout=group_ends)
+        check(lib.dg_m_grouped_bf16_fp4_gemm_ragged(C.byref(args)))
 
 
 # Aliases registered by the reference (csrc/apis/gemm.hpp:922-930)

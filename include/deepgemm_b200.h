@@ -217,6 +217,19 @@ DG_API int dg_k_grouped_fp8_gemm_contiguous(const dg_gemm_args_t* args);
  * scale tensor of D viewed as [m, num_groups * n]).  Rows beyond m are clipped per batch. */
 DG_API int dg_fp8_bmm(const dg_gemm_args_t* args);
 
+/* BF16 activations with E2M1 weights (no counterpart in the reference, whose FP4 GEMMs take quantised activations):
+ *   dg_bf16_fp4_gemm                    D[m, n] (+)= alpha * A[m, k] W[n, k]^T
+ *   dg_m_grouped_bf16_fp4_gemm_ragged   D[r, n]   = A[r, k] W[g(r), n, k]^T, rows sorted by group, groups of any size
+ * a_dtype == DG_BF16, b_dtype == DG_FP4_E2M1_X2, both K-major; b, ldb, sfb, sfb_pitch, gran_k_b describe the weights and
+ * their packed scales exactly as the FP8 x FP4 GEMMs take them (sfa is not used); d_dtype DG_BF16, or DG_FP32 for the dense
+ * form.  k % 128 == 0; a and d 16-byte aligned rows, b 32-byte aligned rows.  accumulate, alpha: dense form only.
+ * ragged: grouped_layout = int32[num_groups] on the device, the row where each group ends; group g is the rows
+ * [grouped_layout[g - 1], grouped_layout[g]) (from row 0 for g = 0) of A [m, k] and D [m, n], with no padding between
+ * groups and no alignment; ends must not decrease; rows at or behind the last end are not written.
+ * Sums are FP32, one rounding per element of D.  A row of A with an infinity or a NaN gives non-finite results. */
+DG_API int dg_bf16_fp4_gemm(const dg_gemm_args_t* args);
+DG_API int dg_m_grouped_bf16_fp4_gemm_ragged(const dg_gemm_args_t* args);
+
 /* Same operation and arguments as dg_fp8_fp4_gemm, for callers that cannot allocate device memory at call time: a
  * serving thread that must never block on the allocator's locks, a process that hands out its whole memory budget at
  * start-up and forbids cudaMalloc afterwards, a plugin host that owns all device memory itself.  It has no counterpart

@@ -1,0 +1,58 @@
+"""bf16_fp4_gemm_nt and m_grouped_bf16_fp4_gemm_nt_ragged without a GPU: what the C ABI refuses before it touches the device, and
+what the Python functions refuse."""
+import ctypes as C
+
+import pytest
+import torch
+
+import deepgemm_amd_b200 as dg
+from deepgemm_amd_b200 import _lib
+
+
+def args(**kw):
+    g = _lib.GemmArgs()
+    fields = dict(a=0x1000, b=0x2000, sfb=0x3000, d=0x4000, m=4, n=64, k=256, num_groups=1, a_dtype=_lib.DG_BF16, b_dtype=_lib.DG_FP4_E2M1_X2,
+                  d_dtype=_lib.DG_BF16, lda=256, ldb=128, ldd=64, sfb_pitch=64, gran_k_b=32)
+    for name, value in {**fields, **kw}.items():
+        setattr(g, name, value)
+    return g
+
+
+REFUSED = [dict(a_dtype=_lib.DG_FP8_E4M3), dict(b_dtype=_lib.DG_BF16), dict(d_dtype=_lib.DG_FP8_E4M3), dict(major_a=1), dict(major_b=1),
+           dict(gran_k_b=64), dict(stochastic_rounding=1), dict(sfd=0x5000), dict(reduce_batches=2), dict(use_psum_layout=1), dict(m=-1),
+           dict(k=192, lda=192, ldb=96), dict(a=None), dict(b=None), dict(sfb=None), dict(d=None), dict(a=0x1008), dict(b=0x2010), dict(sfb=0x3004),
+           dict(d=0x4002), dict(lda=255), dict(lda=248), dict(lda=260), dict(ldb=96), dict(ldb=144), dict(ldd=56), dict(ldd=66), dict(sfb_pitch=60),
+           dict(sfb_pitch=66)]
+
+
+@pytest.mark.parametrize("kw", REFUSED + [dict(num_groups=2), dict(k=0)], ids=str)
+def test_dense_refuses(kw):
+    assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(**kw))) != _lib.DG_OK
+    assert _lib.last_error()
+
+
+@pytest.mark.parametrize("kw", REFUSED + [dict(grouped_layout=None), dict(grouped_layout=0x6002), dict(num_groups=0), dict(num_groups=65536), dict(n=0), dict(k=0),
+                                          dict(accumulate=1), dict(has_alpha=1), dict(d_dtype=_lib.DG_FP32)], ids=str)
+def test_ragged_refuses(kw):
+    assert _lib.lib.dg_m_grouped_bf16_fp4_gemm_ragged(C.byref(args(**{"num_groups": 3, "grouped_layout": 0x6000, **kw}))) != _lib.DG_OK
+    assert _lib.last_error()
+
+
+def test_null_arguments_and_empty_products():
+    for fn in (_lib.lib.dg_bf16_fp4_gemm, _lib.lib.dg_m_grouped_bf16_fp4_gemm_ragged):
+        assert fn(None) != _lib.DG_OK
+    assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(m=0))) == _lib.DG_OK
+    assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(n=0))) == _lib.DG_OK
+
+
+def test_python_functions_refuse_cpu_tensors_and_wrong_shapes():
+    a, w, sf = torch.zeros((4, 256), dtype=torch.bfloat16), torch.zeros((64, 128), dtype=torch.int8), torch.zeros((2, 64), dtype=torch.int).T
+    d = torch.zeros((4, 64), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="Assertion error.*CUDA"):
+        dg.bf16_fp4_gemm_nt(a, (w, sf), d)
+    with pytest.raises(RuntimeError, match="m == m_"):
+        dg.bf16_fp4_gemm_nt(a, (w, sf), d[:3])
+    with pytest.raises(RuntimeError, match="dim"):
+        dg.bf16_fp4_gemm_nt(a[0], (w, sf), d)
+    with pytest.raises(RuntimeError, match="group_ends"):
+        dg.m_grouped_bf16_fp4_gemm_nt_ragged(a, (w.expand(2, 64, 128).contiguous(), sf), d, torch.zeros(2, dtype=torch.int))
