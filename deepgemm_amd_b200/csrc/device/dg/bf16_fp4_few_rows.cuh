@@ -1,0 +1,345 @@
+// D = A W^T for a few BF16 rows of A and packed E2M1 weights W with UE8M0 block scales: the decode form of the BF16 x FP4
+// products.  What bounds it is the bytes of W, half a byte per weight, as long as nothing has to touch every weight.
+//
+// Mathematics.  The tensor cores multiply E2M1 by E4M3 with a power-of-two scale per 32 elements of K on either side
+// (tcgen05.mma.kind::mxf8f6f4), so W goes in as it is.  A BF16 value has 8 significant bits and an E4M3 value 4: every 32 elements
+// of a row of A become two E4M3 vectors with scales s and s / 16,
+//     x = s hi + (s / 16) lo,     hi = e4m3(x / s),  lo = e4m3(16 (x / s - hi)),
+// s being the smallest power of two with |x| / s <= 448.  hi leaves a remainder of at most half its last place, which is a multiple of
+// x's own last place: at most 8 of them, so four bits hold it and the split is exact, down to |x| = 2^-6 s; below that it
+// is off by at most 2^-14 s <= 2^-21 of the block's largest element.  A row of A is thus two columns of the tile, `hi` and `lo`,
+// whose FP32 accumulators are added at the end.  (Unpacking W to FP16 for the register-operand MMA instead costs
+// some 28 instructions per 512 weights, which held a kernel built that way to 3.3 TB/s of W; here no instruction is spent on W.)
+//
+// Work.  W is the 128-row operand: a CTA takes 128 columns of D, up to kTokens rows of A (2 kTokens tile columns) and a share of K.
+//   warp 0      TMA producer: per 128 elements of K 128 rows of W (8 KB, unpacked to a byte each on the way), their scale words, and A
+//   warp 1      MMA issuer
+//   warp 2      allocates tensor memory, rearranges the scale words of W for tcgen05.cp
+//   warps 4-7   split the stage's rows of A into its tile columns and their scales; then the epilogue
+//   warps 8-11  split as well (from 16 rows on)
+// Where the columns of D alone do not occupy the GPU, the CTAs of a cluster (up to 8) share K and send their partial sums to
+// one another through distributed shared memory, every CTA adding up its own rows of D in rank order.  Two CTAs share an SM
+// (up to 32 rows): one's start and end hide behind the other's stream, and the two MMA loops, each bound by its own latency, add up.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ptx.cuh"
+
+namespace dg {
+
+struct Bf16Fp4Params {
+    void* d;                     // [m, n], pitch ldd
+    const int* group_ends;       // null: one group of m rows
+    int* status;                 // host-visible status word, 0 = ok
+    int m, n, k, gran;
+    int64_t ldd;
+    int d_fp32, accumulate;
+    float alpha;
+};
+
+// Rows [first, end) of group g; ends outside [0, m] or before their predecessor give an empty group rather than a wild access
+__device__ __forceinline__ void group_rows(const Bf16Fp4Params& p, int g, int& first, int& end) {
+    first = 0;
+    end = p.m;
+    if (p.group_ends != nullptr) {
+        first = g == 0 ? 0 : min(max(p.group_ends[g - 1], 0), p.m);
+        end = min(max(p.group_ends[g], 0), p.m);
+    }
+}
+
+// One thread's share of the split: eight elements of a row, the four threads of an aligned quad holding 32 consecutive ones.
+// hi, lo: eight E4M3 values each; returns the UE8M0 code of hi's scale (lo's is 4 less), 255 (NaN) for a block with an infinity or NaN.
+__device__ __forceinline__ uint32_t split_bf16(const uint4& raw, uint2& hi, uint2& lo) {
+    const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
+    const uint32_t most2 = __vmaxu2(__vmaxu2(x[0] & 0x7FFF7FFFu, x[1] & 0x7FFF7FFFu), __vmaxu2(x[2] & 0x7FFF7FFFu, x[3] & 0x7FFF7FFFu));
+    uint32_t most = max(most2 & 0xFFFFu, most2 >> 16);                       // the bits of |x| order like |x|
+    most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+    most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+    // |x| = f 2^e with 448 = 1.75 2^8: the code of s is e - 8, one more when f > 1.75.  (Not below 4, so that lo has a code: a block
+    // whose largest element is below 2^-115 is then held to 2^-137)
+    const uint32_t code = max(static_cast<int>((most >> 7) + ((most & 0x7Fu) > 0x60u ? 1u : 0u)) - 8, 4);
+    const __nv_bfloat16 inv = __ushort_as_bfloat16(static_cast<unsigned short>((254u - code) << 7));       // 1 / s
+    uint32_t h[4], l[4];
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x[i]), __halves2bfloat162(inv, inv));      // exact
+        const uint32_t bits = *reinterpret_cast<const uint32_t*>(&y);
+        const __half2 f = __floats2half2_rn(__uint_as_float(bits << 16), __uint_as_float(bits & 0xFFFF0000u));               // |y| <= 448: exact from 2^-17 on
+        uint16_t q;
+        uint32_t back;
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(q) : "r"(*reinterpret_cast<const uint32_t*>(&f)));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(q));
+        const __half2 rest = __hmul2(__hsub2(f, *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(16.0f));
+        uint16_t r;
+        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
+        h[i] = q;
+        l[i] = r;
+    }
+    hi = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    lo = make_uint2(l[0] | (l[1] << 16), l[2] | (l[3] << 16));
+    return most >= 0x7F80u ? 255u : code;
+}
+
+namespace few {
+
+constexpr uint32_t kRoleSplit = 8;           // role code of the splitting warps' waits (status word); the others are the GEMM kernel's
+constexpr int kMaxCluster = 8;
+
+// A bounded wait whose outcome the whole warp shares (some lanes may see the barrier complete just as others give up)
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const AbortCtx& ctx, uint32_t role) {
+    const bool ok = mbar_wait(bar, parity, ctx, role, 1);
+    return __all_sync(0xFFFFFFFFu, ok) != 0;
+}
+
+template <int kTokens> struct Shape {
+    static constexpr int kCols = 2 * kTokens;                                // columns of the tile
+    static constexpr int kCtasPerSm = kTokens <= 16 ? 2 : 1;
+    static constexpr int kStages = kTokens == 8 ? 5 : (kTokens == 16 ? 4 : (kTokens == 32 ? 6 : 3));
+    // The splitting warps form teams that take turns at the K-blocks: a block's chain of wait, shuffles, conversions, stores and fence
+    // is long, so as many blocks as possible are at it at once.  Every lane splits four pieces of eight elements of a block
+    static constexpr int kSplitWarps = kTokens == 8 ? 4 : 8, kTeam = kTokens / 8, kTeams = kSplitWarps / kTeam, kPieces = 4;
+    static constexpr int kThreads = 128 + 32 * kSplitWarps;
+    static_assert(kTeams <= kStages, "a team that is done with its last block knows that the stage of its next one is at most one block behind");
+    static constexpr int kOffB = kStages * 16384, kOffA = kOffB + kStages * kCols * 128, kOffSfa = kOffA + kStages * kTokens * 256, kOffSfb = kOffSfa + kStages * 512;
+    static constexpr int kOffBar = kOffSfb + kStages * 512, kOffMisc = kOffBar + (4 * kStages + 2) * 8, kOffRecv = (kOffMisc + 8 + 15) / 16 * 16;
+    static constexpr int kTmemCols = kCols + 8 <= 32 ? 32 : (kCols + 8 <= 64 ? 64 : (kCols + 8 <= 128 ? 128 : 256));
+    // What a CTA receives: every slice's partial sums of the rows of D it owns
+    __host__ __device__ static constexpr int recv_rows(int slices) { return (kTokens + slices - 1) / slices; }
+    __host__ __device__ static constexpr int smem_bytes(int slices) { return kOffRecv + (slices > 1 ? slices * recv_rows(slices) * 512 : 0); }
+};
+
+template <int kTokens>
+__global__ void __launch_bounds__(Shape<kTokens>::kThreads, Shape<kTokens>::kCtasPerSm)
+bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_sf, const __grid_constant__ CUtensorMap tm_a,
+                         const Bf16Fp4Params p) {
+    using S = Shape<kTokens>;
+    constexpr uint32_t kStages = S::kStages, kCols = S::kCols;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0), lane = lane_id();
+    const uint32_t base = smem_u32(smem);
+    auto full_bar = [&](uint32_t s) { return base + S::kOffBar + s * 8; };
+    auto sf_bar = [&](uint32_t s) { return base + S::kOffBar + (kStages + s) * 8; };
+    auto empty_bar = [&](uint32_t s) { return base + S::kOffBar + (2 * kStages + s) * 8; };
+    auto a_bar = [&](uint32_t s) { return base + S::kOffBar + (3 * kStages + s) * 8; };
+    const uint32_t done_bar = base + S::kOffBar + 4 * kStages * 8, free_bar = done_bar + 8;
+    volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + S::kOffMisc);
+    volatile uint32_t* const abort_flag = tmem_slot + 1;
+    const AbortCtx ctx{abort_flag, p.status};
+    uint32_t slices;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(slices));
+    const uint32_t rank = cluster_ctarank();
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        prefetch_tensormap(&tm_w);
+        prefetch_tensormap(&tm_sf);
+        prefetch_tensormap(&tm_a);
+    }
+    if (warp == 1 && lane == 0) {
+        for (uint32_t s = 0; s < kStages; ++s) {
+            mbar_init(full_bar(s), 2 + S::kTeam);    // the producer, the rearranging warp, a team of splitting warps
+            mbar_init(sf_bar(s), 1);
+            mbar_init(empty_bar(s), 1);          // tcgen05.commit
+            mbar_init(a_bar(s), 1);
+        }
+        mbar_init(done_bar, 1);                  // tcgen05.commit: a pass's accumulators are complete
+        mbar_init(free_bar, 4);                  // the epilogue warps have read them
+        fence_mbar_init();
+    }
+    __syncwarp();
+    if (warp == 2) {
+        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
+        tmem_relinquish<1>();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot, tmem_sfa = tmem + kCols, tmem_sfb = tmem_sfa + 4;
+    griddep_wait();
+    griddep_launch_dependents();
+
+    const int group = blockIdx.z, n0 = blockIdx.x / slices * 128;
+    int first, end;
+    group_rows(p, group, first, end);
+    const int num_blocks = p.k / 128, per_slice = (num_blocks + slices - 1) / slices;
+    const int kb0 = min(static_cast<int>(rank) * per_slice, num_blocks), kb1 = min(kb0 + per_slice, num_blocks);
+    uint32_t stage = 0, phase = 0;
+    auto advance = [&]() {
+        stage = stage + 1 == kStages ? 0 : stage + 1;
+        phase ^= stage == 0;
+    };
+    bool ok = true;
+
+    // Every role walks the same passes (kTokens rows of A each) and K-blocks
+    uint32_t pass = 0, steps = 0;                // (steps: K-blocks of the passes before, for the splitting warps)
+    for (int r0 = first + blockIdx.y * kTokens; r0 < end; r0 += gridDim.y * kTokens, ++pass) {
+        // first half of a split barrier: this CTA runs, and what it received in the pass before has been read
+        __syncwarp();
+        if (slices > 1) cluster_arrive_relaxed();
+        if (warp == 0) {
+            for (int kb = kb0; ok && kb < kb1; ++kb, advance()) {
+                if (!(ok = warp_wait(empty_bar(stage), phase ^ 1, ctx, 1))) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(a_bar(stage), kTokens * 256);
+                    tma_load_2d(base + S::kOffA + stage * kTokens * 256, &tm_a, a_bar(stage), kb * 128, r0);
+                    mbar_arrive_expect_tx(sf_bar(stage), 512);
+                    tma_load_2d(base + S::kOffSfa + stage * 512, &tm_sf, sf_bar(stage), n0,
+                                group * ((p.k + 4 * p.gran - 1) / (4 * p.gran)) + (p.gran == 32 ? kb : kb / 4));
+                    mbar_arrive_expect_tx(full_bar(stage), 128 * 64);
+                    tma_load_2d(base + stage * 16384, &tm_w, full_bar(stage), kb * 128, group * p.n + n0);
+                }
+                __syncwarp();
+            }
+        } else if (warp == 1) {
+            constexpr uint32_t idesc = make_instr_desc_block_scaled(kFmtE2M1, kFmtE4M3, 0, 0, 128, kCols);
+            ok = ok && warp_wait(free_bar, (pass & 1) ^ 1, ctx, 2);
+            tc_fence_after_sync();
+            for (int kb = kb0; ok && kb < kb1; ++kb, advance()) {
+                if (!(ok = warp_wait(full_bar(stage), phase, ctx, 2))) break;
+                tc_fence_after_sync();
+                if (lane == 0) {
+                    tc_cp_32x128b_warpx4<1>(tmem_sfa, make_smem_desc(base + S::kOffSfa + stage * 512, 0, 128, kSwizzleNone));
+                    tc_cp_32x128b_warpx4<1>(tmem_sfb, make_smem_desc(base + S::kOffSfb + stage * 512, 0, 128, kSwizzleNone));
+                    const uint64_t a_desc = make_smem_desc(base + stage * 16384, 0, 1024, kSwizzle128B);
+                    const uint64_t b_desc = make_smem_desc(base + S::kOffB + stage * kCols * 128, 0, 1024, kSwizzle128B);
+                    #pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j)
+                        tc_mma_mxf8f6f4<1>(tmem, a_desc + j * 2, b_desc + j * 2, instr_desc_with_sf_ids(idesc, p.gran == 32 ? j : kb % 4, j), tmem_sfa, tmem_sfb,
+                                           kb != kb0 || j != 0);
+                    tc_commit(empty_bar(stage));
+                    if (kb + 1 == kb1) tc_commit(done_bar);
+                }
+                __syncwarp();
+            }
+        } else if (warp == 2) {
+            // tcgen05.cp puts row r of 32 x 16 bytes into lane r: the word of tile row 32 c + r has to sit at word 4 r + c
+            for (int kb = kb0; ok && kb < kb1; ++kb, advance()) {
+                if (!(ok = warp_wait(sf_bar(stage), phase, ctx, 3))) break;
+                const uint32_t words = base + S::kOffSfa + stage * 512;
+                uint32_t v[4];
+                #pragma unroll
+                for (uint32_t c = 0; c < 4; ++c) v[c] = ld_shared_u32(words + (c * 32 + lane) * 4);
+                __syncwarp();
+                st_shared_v4(words + lane * 16, v[0], v[1], v[2], v[3]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full_bar(stage));
+            }
+        } else if (warp >= 4) {
+            const int rows = min(kTokens, end - r0), blocks = kb1 - kb0;
+            const int team = (warp - 4) / S::kTeam, member = (warp - 4) % S::kTeam;
+            // Piece i of this lane: elements 8 (lane % 16) .. of the K-block, of row 2 (i kTeam + member) + lane / 16
+            const int row0 = member * 2 + lane / 16, chunk = lane % 16;
+            for (int b = team; ok && b < blocks; b += S::kTeams) {
+                const uint32_t at_stage = (steps + b) % kStages, at_phase = (steps + b) / kStages & 1;
+                // First that the stage's block before this one has been multiplied, then that this one's A has landed.  Copies land in any
+                // order, and a team that only asked for the latter could ask while the copy of the block before is still
+                // under way: a barrier two phases behind answers like one that is done.
+                if (!(ok = warp_wait(empty_bar(at_stage), at_phase ^ 1, ctx, kRoleSplit))) break;
+                if (!(ok = warp_wait(a_bar(at_stage), at_phase, ctx, kRoleSplit))) break;
+                const uint8_t* const a = smem + S::kOffA + at_stage * kTokens * 256 + chunk * 16;
+                uint8_t* const tile = smem + S::kOffB + at_stage * kCols * 128;
+                uint8_t* const sf = smem + S::kOffSfb + at_stage * 512;
+                #pragma unroll
+                for (int i = 0; i < S::kPieces; ++i) {
+                    if (2 * (S::kTeam * i + member) < rows) {                // (a row beyond the last one beside it: its columns are not stored)
+                        const int row = row0 + 2 * S::kTeam * i, col = kTokens + row;
+                        uint2 hi, lo;
+                        const uint32_t code = split_bf16(*reinterpret_cast<const uint4*>(a + row * 256), hi, lo);
+                        const int at = (((chunk / 2) ^ (row & 7)) << 4) + chunk % 2 * 8;
+                        *reinterpret_cast<uint2*>(tile + row * 128 + at) = hi;
+                        *reinterpret_cast<uint2*>(tile + col * 128 + at) = lo;
+                        if (chunk % 4 == 0) {
+                            sf[row % 32 * 16 + row / 32 * 4 + chunk / 4] = static_cast<uint8_t>(code);
+                            sf[col % 32 * 16 + col / 32 * 4 + chunk / 4] = static_cast<uint8_t>(code == 255 ? 255 : code - 4);
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full_bar(at_stage));
+            }
+            steps += blocks;
+        }
+        if (warp >= 4 && warp < 8) {
+            const int rows = min(kTokens, end - r0);
+            // Epilogue: this thread's column of D, rows r0 .. r0 + rows
+            const uint32_t quarter = warp % 4, row = quarter * 32 + lane;
+            const int n = n0 + static_cast<int>(row);
+            auto write = [&](int t, float y) {
+                if (t >= rows || n >= p.n) return;
+                const int64_t at = static_cast<int64_t>(r0 + t) * p.ldd + n;
+                y *= p.alpha;
+                if (p.d_fp32) {
+                    float* const out = static_cast<float*>(p.d) + at;
+                    *out = p.accumulate ? *out + y : y;
+                } else {
+                    __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.d) + at;
+                    if (p.accumulate) y += __bfloat162float(*out);
+                    *out = __float2bfloat16_rn(y);
+                }
+            };
+            const bool some = kb1 > kb0;                                     // (a slice beyond the end of K has nothing to add)
+            if (ok && some) ok = warp_wait(done_bar, pass & 1, ctx, 4);
+            tc_fence_after_sync();
+            const uint32_t own_rows = S::recv_rows(slices), recv = base + S::kOffRecv;
+            __syncwarp();
+            if (slices > 1) cluster_wait();                                  // every CTA of the cluster may be written to
+            #pragma unroll
+            for (int t0 = 0; t0 < kTokens; t0 += 16) {
+                uint32_t v[16], w[16];
+                __syncwarp();                                                // (lanes beyond N skip the stores)
+                if (some) {
+                    tmem_ld_32x32b_x16(tmem + ((quarter * 32) << 16) + t0, v);
+                    if constexpr (kTokens >= 16) tmem_ld_32x32b_x16(tmem + ((quarter * 32) << 16) + kTokens + t0, w);
+                    tmem_ld_wait();
+                }
+                #pragma unroll
+                for (int i = 0; i < (kTokens < 16 ? kTokens : 16); ++i) {
+                    const int t = t0 + i;
+                    const float y = !some ? 0.0f : __uint_as_float(v[i]) + __uint_as_float(kTokens >= 16 ? w[i] : v[i + 8]);
+                    if (slices == 1) write(t, y);
+                    else if (t < rows) st_shared_cluster_u32(map_to_cta(recv + ((rank * own_rows + t / slices) * 128 + row) * 4, t % slices), __float_as_uint(y));
+                }
+            }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(free_bar);
+            __syncwarp();                                                    // (the cluster barrier wants the warp together)
+            if (slices > 1) {
+                cluster_arrive();                                            // release: what this CTA sent is visible to its owners
+                cluster_wait();
+                for (uint32_t i = 0; i < own_rows; ++i) {
+                    const int t = static_cast<int>(i * slices + rank);
+                    if (t >= rows) break;
+                    float y = 0.0f;
+                    for (uint32_t s = 0; s < slices; ++s) y += __uint_as_float(ld_shared_u32(recv + ((s * own_rows + i) * 128 + row) * 4));
+                    write(t, y);
+                }
+            }
+        }
+        if (slices > 1 && (warp < 4 || warp >= 8)) {
+            // the other warps only take part in the two barriers of the epilogue
+            __syncwarp();
+            cluster_wait();
+            cluster_arrive();
+            cluster_wait();
+        }
+    }
+
+    __syncthreads();
+    if (*abort_flag != 0) {                      // a wait ran out: copies still in flight get time to land
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 200000) { }
+        __syncthreads();
+    }
+    if (warp == 2) {
+        tc_fence_after_sync();
+        tmem_dealloc<1>(tmem, S::kTmemCols);
+    }
+}
+
+}  // namespace few
+}  // namespace dg

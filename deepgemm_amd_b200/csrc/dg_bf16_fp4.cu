@@ -8,99 +8,54 @@
 // those of the FP32 sums and the one of the result.
 #include "dg_common.hpp"
 
-#include <cuda_bf16.h>
-
 #include <algorithm>
+
+#include "device/dg/bf16_fp4_few_rows.cuh"
 
 namespace dg {
 namespace {
 
-struct Bf16Fp4Params {
-    const __nv_bfloat16* a;      // [m, k], pitch lda
-    const uint8_t* w;            // [groups, n, k / 2], pitch ldb
-    const uint32_t* sf;          // [groups][ceil(k / (4 gran))][sf_pitch]
-    void* d;                     // [m, n], pitch ldd
-    const int* group_ends;       // null: one group of m rows
-    int m, n, k, gran;
-    int64_t lda, ldb, ldd, sf_pitch;
-    int accumulate;
-    float alpha;
-};
-
-// Rows [first, end) of group g; ends outside [0, m] or before their predecessor give an empty group rather than a wild access
-__device__ __forceinline__ void group_rows(const Bf16Fp4Params& p, int g, int& first, int& end) {
-    first = 0;
-    end = p.m;
-    if (p.group_ends != nullptr) {
-        first = g == 0 ? 0 : min(max(p.group_ends[g - 1], 0), p.m);
-        end = min(max(p.group_ends[g], 0), p.m);
-    }
+// CTAs along K (a cluster) of a launch with `tiles` CTAs of 128 columns: enough to occupy the GPU, as long as each keeps four K-blocks
+int choose_slices(int64_t tiles, int ctas_per_sm, int num_blocks) {
+    const int64_t slots = static_cast<int64_t>(dg_get_num_sms()) * ctas_per_sm;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({few::kMaxCluster, slots / tiles, num_blocks / 4})));
 }
 
-// UE8M0 code -> FP32: code 0 is 2^-127 (an FP32 subnormal), code 255 has no value (infinity here, so the result shows it)
-__device__ __forceinline__ float ue8m0_value(uint32_t code) { return __uint_as_float(max(code << 23, 0x00400000u)); }
-
-__device__ __forceinline__ float e2m1_value(uint32_t code) {
-    const uint32_t e = (code >> 1) & 3, m = code & 1;
-    const float size = e == 0 ? 0.5f * m : (1.0f + 0.5f * m) * static_cast<float>(1 << (e - 1));
-    return code & 8 ? -size : size;
-}
-
-// One warp per column of D and up to eight rows: the lanes share K in words of eight weights, the sums meet by shuffles.
-constexpr int kRowsPerPass = 8;
-
-template <bool kDIsFP32>
-__global__ void __launch_bounds__(256) bf16_fp4_kernel(const Bf16Fp4Params p) {
-    const int lane = threadIdx.x % 32, n = blockIdx.x * 8 + threadIdx.x / 32, g = blockIdx.z;
-    if (n >= p.n) return;
-    int first, end;
-    group_rows(p, g, first, end);
-    const uint8_t* w = p.w + (static_cast<int64_t>(g) * p.n + n) * p.ldb;
-    const int words = (p.k + 4 * p.gran - 1) / (4 * p.gran);
-    const uint32_t* sf = p.sf + static_cast<int64_t>(g) * words * p.sf_pitch + n;
-    for (int r0 = first + blockIdx.y * kRowsPerPass; r0 < end; r0 += gridDim.y * kRowsPerPass) {
-        const int rows = min(kRowsPerPass, end - r0);
-        float sum[kRowsPerPass] = {};
-        for (int k0 = lane * 8; k0 < p.k; k0 += 256) {
-            const uint32_t codes = *reinterpret_cast<const uint32_t*>(w + k0 / 2);
-            const int block = k0 / p.gran;
-            const float scale = ue8m0_value((sf[static_cast<int64_t>(block / 4) * p.sf_pitch] >> (8 * (block % 4))) & 0xFFu);
-            float v[8];
-            #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = e2m1_value((codes >> (4 * i)) & 15u);
-            #pragma unroll
-            for (int r = 0; r < kRowsPerPass; ++r) {
-                if (r >= rows) break;
-                const uint4 raw = *reinterpret_cast<const uint4*>(p.a + static_cast<int64_t>(r0 + r) * p.lda + k0);
-                const uint32_t pair[4] = {raw.x, raw.y, raw.z, raw.w};
-                float part = 0.0f;
-                #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    part = fmaf(__uint_as_float(pair[i] << 16), v[2 * i], part);
-                    part = fmaf(__uint_as_float(pair[i] & 0xFFFF0000u), v[2 * i + 1], part);
-                }
-                sum[r] = fmaf(part, scale, sum[r]);
-            }
-        }
-        #pragma unroll
-        for (int r = 0; r < kRowsPerPass; ++r) {
-            if (r >= rows) break;
-            #pragma unroll
-            for (int off = 16; off > 0; off /= 2) sum[r] += __shfl_xor_sync(0xFFFFFFFFu, sum[r], off);
-            if (lane == 0) {
-                const int64_t at = static_cast<int64_t>(r0 + r) * p.ldd + n;
-                float x = sum[r] * p.alpha;
-                if constexpr (kDIsFP32) {
-                    float* out = static_cast<float*>(p.d) + at;
-                    *out = p.accumulate ? *out + x : x;
-                } else {
-                    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.d) + at;
-                    if (p.accumulate) x += __bfloat162float(*out);
-                    *out = __float2bfloat16_rn(x);
-                }
-            }
-        }
+template <int kTokens>
+int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p) {
+    using S = few::Shape<kTokens>;
+    const int tiles_n = ceil_div(g->n, 128), passes = p.group_ends != nullptr ? 1 : ceil_div(g->m, kTokens);
+    const int slices = choose_slices(static_cast<int64_t>(tiles_n) * passes * g->num_groups, S::kCtasPerSm, g->k / 128);
+    CUtensorMap tm_w, tm_sf, tm_a;
+    int rc;
+    const uint64_t words = ceil_div(g->k, 4 * g->gran_k_b);
+    if ((rc = encode_tensor_map_2d(&tm_w, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, g->b, g->k, static_cast<uint64_t>(g->num_groups) * g->n, g->ldb, 128, 128,
+                                   CU_TENSOR_MAP_SWIZZLE_128B)) != DG_OK) return rc;
+    if ((rc = encode_tensor_map_2d(&tm_sf, CU_TENSOR_MAP_DATA_TYPE_INT32, g->sfb, g->n, words * g->num_groups, g->sfb_pitch * 4, 128, 1,
+                                   CU_TENSOR_MAP_SWIZZLE_NONE)) != DG_OK) return rc;
+    if ((rc = encode_tensor_map_2d(&tm_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g->a, g->k, g->m, g->lda * 2, 128, kTokens, CU_TENSOR_MAP_SWIZZLE_NONE)) != DG_OK) return rc;
+    const auto kernel = few::bf16_fp4_few_rows_kernel<kTokens>;
+    const int smem = S::smem_bytes(slices);
+    DG_CUDA_RT(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(tiles_n * slices, passes, g->num_groups);
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(g->stream);
+    cudaLaunchAttribute attrs[2];
+    if (slices > 1) {
+        attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[cfg.numAttrs].val.clusterDim.x = slices;
+        attrs[cfg.numAttrs].val.clusterDim.y = attrs[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
     }
+    if (state().pdl) {
+        attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attrs;
+    DG_CUDA_RT(cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_sf, tm_a, p));
+    return DG_OK;
 }
 
 int run(const dg_gemm_args_t* g, bool ragged) {
@@ -126,15 +81,15 @@ int run(const dg_gemm_args_t* g, bool ragged) {
     DG_REQUIRE(g->ldd >= g->n && (g->ldd * d_elem) % 16 == 0);
     DG_REQUIRE(g->sfb_pitch >= align_up<int64_t>(g->n, 4) && g->sfb_pitch % 4 == 0);
 
-    const Bf16Fp4Params p{static_cast<const __nv_bfloat16*>(g->a), static_cast<const uint8_t*>(g->b), static_cast<const uint32_t*>(g->sfb), g->d,
-                          ragged ? g->grouped_layout : nullptr, g->m, g->n, g->k, g->gran_k_b, g->lda, g->ldb, g->ldd, g->sfb_pitch,
-                          g->accumulate != 0, g->has_alpha ? g->alpha : 1.0f};
-    const dim3 grid(ceil_div(g->n, 8), std::min(ceil_div(g->m, kRowsPerPass), ragged ? 8 : 1024), g->num_groups);
-    const auto stream = static_cast<cudaStream_t>(g->stream);
-    if (g->d_dtype == DG_FP32) bf16_fp4_kernel<true><<<grid, 256, 0, stream>>>(p);
-    else bf16_fp4_kernel<false><<<grid, 256, 0, stream>>>(p);
-    DG_CUDA_RT(cudaGetLastError());
-    return DG_OK;
+    int rc = ensure_status_word();
+    if (rc != DG_OK) return rc;
+    const Bf16Fp4Params p{g->d, ragged ? g->grouped_layout : nullptr, state().status_device, g->m, g->n, g->k, g->gran_k_b,
+                          g->ldd, g->d_dtype == DG_FP32, g->accumulate != 0, g->has_alpha ? g->alpha : 1.0f};
+    const int rows = ragged ? ceil_div(g->m, g->num_groups) : g->m;
+    if (rows <= 8) return launch_few_rows<8>(g, p);
+    if (rows <= 16) return launch_few_rows<16>(g, p);
+    if (rows <= 32) return launch_few_rows<32>(g, p);
+    return launch_few_rows<64>(g, p);
 }
 
 }  // namespace

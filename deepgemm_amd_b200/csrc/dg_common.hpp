@@ -80,6 +80,9 @@ State& state();
 int device_num_sms();                // SM count of the current device, 0 if there is none
 int ensure_status_word();            // allocates the host-mapped status word on first GPU use
 void release_split_workspaces();     // frees the library-owned split-K panels of every device
+// A tiled tensor map over [outer][inner] elements with rows outer_stride_bytes apart (dg_gemm.cpp; the last maps are kept per thread)
+int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t outer, uint64_t outer_stride_bytes,
+                         uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle);
 #define DG_REQUIRE_ALIVE() \
     do { if (::dg::state().shut_down) return ::dg::fail(DG_ERR_INVALID_ARGUMENT, "the runtime has been shut down (dg_shutdown)"); } while (0)
 

@@ -922,6 +922,11 @@ int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratc
 
 }  // namespace
 
+int encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t outer, uint64_t outer_stride_bytes,
+                         uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
+    return encode_2d(map, dtype, base, inner, outer, outer_stride_bytes, box_inner, box_outer, swizzle);
+}
+
 void release_split_workspaces() {
     std::lock_guard<std::mutex> lock(g_workspace_mu);
     for (auto& [device, w] : g_workspaces)
