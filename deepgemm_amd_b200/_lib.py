@@ -78,8 +78,9 @@ SIGNATURES = {
     "dg_m_grouped_fp8_fp4_gemm_masked": (C.c_int, [C.POINTER(GemmArgs)]),
     "dg_k_grouped_fp8_gemm_contiguous": (C.c_int, [C.POINTER(GemmArgs)]),
     "dg_fp8_bmm": (C.c_int, [C.POINTER(GemmArgs)]),
-    "dg_bf16_fp4_gemm": (C.c_int, [C.POINTER(GemmArgs)]),
-    "dg_m_grouped_bf16_fp4_gemm_ragged": (C.c_int, [C.POINTER(GemmArgs)]),
+    "dg_bf16_fp4_workspace_bytes": (C.c_int64, [C.POINTER(GemmArgs), C.c_int]),
+    "dg_bf16_fp4_gemm": (C.c_int, [C.POINTER(GemmArgs), C.c_void_p, C.c_int64]),
+    "dg_m_grouped_bf16_fp4_gemm_ragged": (C.c_int, [C.POINTER(GemmArgs), C.c_void_p, C.c_int64]),
     "dg_gemm_precompile": (C.c_int, [C.c_int, C.POINTER(GemmArgs)]),
     "dg_get_gemm_config": (C.c_int, [C.c_int, C.POINTER(GemmArgs), C.POINTER(GemmConfig)]),
     "dg_enumerate_tiles": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,

@@ -1094,6 +1094,13 @@ def _bf16_fp4_args(a, b, d, n, k, groups, recipe_b, **kw) -> GemmArgs:
     return args
 
 
+def _run_bf16_fp4(fn, args: GemmArgs, ragged: bool, device) -> None:
+    size = lib.dg_bf16_fp4_workspace_bytes(C.byref(args), int(ragged))
+    # the call's own: PyTorch's allocator hands it to another stream, or a captured graph's pool to another graph, only with the order kept
+    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
+    check(fn(C.byref(args), workspace.data_ptr() if workspace is not None else None, size))
+
+
 def _on_device_of(t: torch.Tensor):
     """The calls below launch on the device their tensors live on, whichever device is current."""
     return torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
@@ -1104,6 +1111,8 @@ def bf16_fp4_gemm_nt(a, b, d, c=None, recipe_b=(1, 32), compiled_dims: str = "nk
     weights an FP8 x FP4 GEMM takes, in the same storage, multiplied with activations that are not quantised.  recipe_b =
     (1, 32) or (1, 128); scales packed (int32) or FP32 (packed on the fly); D BF16 or FP32; K % 128 == 0.  Any number of
     rows from a single token on; sums in FP32, one rounding per element (two where C is added to a BF16 D)."""
+    if _C is not None and _C.bf16_fp4(a, b, d, c, None, recipe_b, alpha):
+        return
     w, _ = b
     _require(a.dim() == 2 and w.dim() == 2 and d.dim() == 2, "t.dim() == N")
     (m, k), n = a.shape, w.size(0)
@@ -1125,7 +1134,7 @@ def bf16_fp4_gemm_nt(a, b, d, c=None, recipe_b=(1, 32), compiled_dims: str = "nk
         args = _bf16_fp4_args(a, b, d, n, k, 1, recipe_b, accumulate=c is not None, alpha=alpha)
         if c is not None and not is_cd_same:
             d.copy_(c)
-        check(lib.dg_bf16_fp4_gemm(C.byref(args)))
+        _run_bf16_fp4(lib.dg_bf16_fp4_gemm, args, False, d.device)
 
 
 def m_grouped_bf16_fp4_gemm_nt_ragged(a, b, d, group_ends, recipe_b=(1, 32), compiled_dims: str = "nk") -> None:
@@ -1133,6 +1142,8 @@ def m_grouped_bf16_fp4_gemm_nt_ragged(a, b, d, group_ends, recipe_b=(1, 32), com
     scales): the expert layer of the 4-bit weights above.  group_ends (int32 [G], on the device, not decreasing) holds the
     row where each group ends; the groups follow one another without padding or alignment, empty ones included, and rows
     at or behind group_ends[-1] keep what D holds.  Capturable: a replay follows the ends of that moment.  D BF16."""
+    if _C is not None and _C.bf16_fp4(a, b, d, None, group_ends, recipe_b, None):
+        return
     w, _ = b
     _require(a.dim() == 2 and w.dim() == 3 and d.dim() == 2, "t.dim() == N")
     (m, k), (groups, n, _) = a.shape, w.shape
@@ -1146,7 +1157,7 @@ def m_grouped_bf16_fp4_gemm_nt_ragged(a, b, d, group_ends, recipe_b=(1, 32), com
         return
     with _on_device_of(d):
         args = _bf16_fp4_args(a, b, d, n, k, groups, recipe_b, layout=group_ends)
-        check(lib.dg_m_grouped_bf16_fp4_gemm_ragged(C.byref(args)))
+        _run_bf16_fp4(lib.dg_m_grouped_bf16_fp4_gemm_ragged, args, True, d.device)
 
 
 # Aliases registered by the reference (csrc/apis/gemm.hpp:922-930)

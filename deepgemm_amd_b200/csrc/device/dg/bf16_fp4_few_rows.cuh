@@ -16,7 +16,8 @@
 //   warp 1      MMA issuer
 //   warp 2      allocates tensor memory, rearranges the scale words of W for tcgen05.cp
 //   warps 4-7   split the stage's rows of A into its tile columns and their scales; then the epilogue
-//   warps 8-11  split as well (from 16 rows on)
+// From nine rows on splitting them again in every CTA costs more than the weights (a block of 32 rows took 0.6 us), so a kernel of its own
+// does it once and this one loads the two planes; it asks for the first stages of W before that kernel is done.
 // Where the columns of D alone do not occupy the GPU, the CTAs of a cluster (up to 8) share K and send their partial sums to
 // one another through distributed shared memory, every CTA adding up its own rows of D in rank order.  Two CTAs share an SM
 // (up to 32 rows): one's start and end hide behind the other's stream, and the two MMA loops, each bound by its own latency, add up.
@@ -29,6 +30,11 @@
 
 namespace dg {
 
+// The rows of A split ahead of the product (dg_bf16_fp4.cu) lie in slots: those of group g from a multiple of four on, so that a TMA
+// copy of their scale words may start there.  Groups keep their order and do not overlap: the next one's first slot is behind the last row
+// of this one's, whatever its size.
+__host__ __device__ __forceinline__ int first_slot(int first_row, int group) { return (first_row + 3) / 4 * 4 + 4 * group; }
+
 struct Bf16Fp4Params {
     void* d;                     // [m, n], pitch ldd
     const int* group_ends;       // null: one group of m rows
@@ -37,6 +43,7 @@ struct Bf16Fp4Params {
     int64_t ldd;
     int d_fp32, accumulate;
     float alpha;
+    int slots;                   // A split ahead: slots per plane (hi, then lo)
 };
 
 // Rows [first, end) of group g; ends outside [0, m] or before their predecessor give an empty group rather than a wild access
@@ -93,16 +100,17 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const A
     return __all_sync(0xFFFFFFFFu, ok) != 0;
 }
 
-template <int kTokens> struct Shape {
+// kSplit: the kernel splits A itself (a token or a few); otherwise A comes as the two planes of a kernel before this one
+template <int kTokens, bool kSplit> struct Shape {
     static constexpr int kCols = 2 * kTokens;                                // columns of the tile
-    static constexpr int kCtasPerSm = kTokens <= 16 ? 2 : 1;
-    static constexpr int kStages = kTokens == 8 ? 5 : (kTokens == 16 ? 4 : (kTokens == 32 ? 6 : 3));
+    static constexpr int kCtasPerSm = kTokens <= 32 ? 2 : 1;
+    static constexpr int kStages = kTokens == 8 ? 5 : (kTokens == 16 ? 4 : (kTokens == 32 ? 3 : 5));
     // The splitting warps form teams that take turns at the K-blocks: a block's chain of wait, shuffles, conversions, stores and fence
     // is long, so as many blocks as possible are at it at once.  Every lane splits four pieces of eight elements of a block
-    static constexpr int kSplitWarps = kTokens == 8 ? 4 : 8, kTeam = kTokens / 8, kTeams = kSplitWarps / kTeam, kPieces = 4;
-    static constexpr int kThreads = 128 + 32 * kSplitWarps;
-    static_assert(kTeams <= kStages, "a team that is done with its last block knows that the stage of its next one is at most one block behind");
-    static constexpr int kOffB = kStages * 16384, kOffA = kOffB + kStages * kCols * 128, kOffSfa = kOffA + kStages * kTokens * 256, kOffSfb = kOffSfa + kStages * 512;
+    static constexpr int kTeam = kTokens / 8, kTeams = 4 / kTeam, kPieces = 4;
+    static constexpr int kThreads = 256;
+    static_assert(!kSplit || (kTeams >= 1 && kTeams <= kStages), "a team that is done with its last block knows that the stage of its next one is at most one block behind");
+    static constexpr int kOffB = kStages * 16384, kOffA = kOffB + kStages * kCols * 128, kOffSfa = kOffA + (kSplit ? kStages * kTokens * 256 : 0), kOffSfb = kOffSfa + kStages * 512;
     static constexpr int kOffBar = kOffSfb + kStages * 512, kOffMisc = kOffBar + (4 * kStages + 2) * 8, kOffRecv = (kOffMisc + 8 + 15) / 16 * 16;
     static constexpr int kTmemCols = kCols + 8 <= 32 ? 32 : (kCols + 8 <= 64 ? 64 : (kCols + 8 <= 128 ? 128 : 256));
     // What a CTA receives: every slice's partial sums of the rows of D it owns
@@ -110,11 +118,11 @@ template <int kTokens> struct Shape {
     __host__ __device__ static constexpr int smem_bytes(int slices) { return kOffRecv + (slices > 1 ? slices * recv_rows(slices) * 512 : 0); }
 };
 
-template <int kTokens>
-__global__ void __launch_bounds__(Shape<kTokens>::kThreads, Shape<kTokens>::kCtasPerSm)
+template <int kTokens, bool kSplit>
+__global__ void __launch_bounds__(256, Shape<kTokens, kSplit>::kCtasPerSm)
 bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_sf, const __grid_constant__ CUtensorMap tm_a,
-                         const Bf16Fp4Params p) {
-    using S = Shape<kTokens>;
+                         const __grid_constant__ CUtensorMap tm_sfa, const Bf16Fp4Params p) {
+    using S = Shape<kTokens, kSplit>;
     constexpr uint32_t kStages = S::kStages, kCols = S::kCols;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0), lane = lane_id();
@@ -136,10 +144,11 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
         prefetch_tensormap(&tm_w);
         prefetch_tensormap(&tm_sf);
         prefetch_tensormap(&tm_a);
+        if (!kSplit) prefetch_tensormap(&tm_sfa);
     }
     if (warp == 1 && lane == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
-            mbar_init(full_bar(s), 2 + S::kTeam);    // the producer, the rearranging warp, a team of splitting warps
+            mbar_init(full_bar(s), 2 + (kSplit ? S::kTeam : 0));      // the producer, the rearranging warp, a team of splitting warps
             mbar_init(sf_bar(s), 1);
             mbar_init(empty_bar(s), 1);          // tcgen05.commit
             mbar_init(a_bar(s), 1);
@@ -157,7 +166,9 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot, tmem_sfa = tmem + kCols, tmem_sfb = tmem_sfa + 4;
-    griddep_wait();
+    // With A split ahead, what the kernel before this one wrote is A alone: the producer asks for W before it waits for that kernel (it was
+    // itself launched behind everything that came before)
+    if (kSplit || warp != 0) griddep_wait();
     griddep_launch_dependents();
 
     const int group = blockIdx.z, n0 = blockIdx.x / slices * 128;
@@ -179,16 +190,44 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
         __syncwarp();
         if (slices > 1) cluster_arrive_relaxed();
         if (warp == 0) {
-            for (int kb = kb0; ok && kb < kb1; ++kb, advance()) {
-                if (!(ok = warp_wait(empty_bar(stage), phase ^ 1, ctx, 1))) break;
-                if (lane == 0) {
+            const int sf_row = group * ((p.k + 4 * p.gran - 1) / (4 * p.gran));
+            auto load_w = [&](int kb) {
+                mbar_arrive_expect_tx(sf_bar(stage), 512 + (kSplit ? 0 : kCols * 4));
+                tma_load_2d(base + S::kOffSfa + stage * 512, &tm_sf, sf_bar(stage), n0, sf_row + (p.gran == 32 ? kb : kb / 4));
+                mbar_arrive_expect_tx(full_bar(stage), 128 * 64 + (kSplit ? 0 : kCols * 128));
+                tma_load_2d(base + stage * 16384, &tm_w, full_bar(stage), kb * 128, group * p.n + n0);
+            };
+            auto load_a = [&](int kb) {
+                if constexpr (kSplit) {
                     mbar_arrive_expect_tx(a_bar(stage), kTokens * 256);
                     tma_load_2d(base + S::kOffA + stage * kTokens * 256, &tm_a, a_bar(stage), kb * 128, r0);
-                    mbar_arrive_expect_tx(sf_bar(stage), 512);
-                    tma_load_2d(base + S::kOffSfa + stage * 512, &tm_sf, sf_bar(stage), n0,
-                                group * ((p.k + 4 * p.gran - 1) / (4 * p.gran)) + (p.gran == 32 ? kb : kb / 4));
-                    mbar_arrive_expect_tx(full_bar(stage), 128 * 64);
-                    tma_load_2d(base + stage * 16384, &tm_w, full_bar(stage), kb * 128, group * p.n + n0);
+                } else {
+                    const int slot = (p.group_ends != nullptr ? first_slot(first, group) : 0) + r0 - first;
+                    tma_load_2d(base + S::kOffSfb + stage * 512, &tm_sfa, sf_bar(stage), slot, 2 * kb);      // hi's words, then lo's
+                    #pragma unroll
+                    for (int plane = 0; plane < 2; ++plane)
+                        tma_load_2d(base + S::kOffB + stage * kCols * 128 + plane * kTokens * 128, &tm_a, full_bar(stage), kb * 128, plane * p.slots + slot);
+                }
+            };
+            int kb = kb0;
+            if (!kSplit && pass == 0) {
+                // every stage is free: W for all of them, then the kernel before this one, then A
+                const int ahead = min(kb0 + static_cast<int>(kStages), kb1);
+                for (; kb < ahead; ++kb, advance())
+                    if (lane == 0) load_w(kb);
+                __syncwarp();
+                griddep_wait();
+                stage = 0;
+                for (int b = kb0; b < ahead; ++b, ++stage)
+                    if (lane == 0) load_a(b);
+                stage = (ahead - kb0) % kStages;
+                __syncwarp();
+            }
+            for (; ok && kb < kb1; ++kb, advance()) {
+                if (!(ok = warp_wait(empty_bar(stage), phase ^ 1, ctx, 1))) break;
+                if (lane == 0) {
+                    load_w(kb);
+                    load_a(kb);
                 }
                 __syncwarp();
             }
@@ -223,11 +262,18 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                 for (uint32_t c = 0; c < 4; ++c) v[c] = ld_shared_u32(words + (c * 32 + lane) * 4);
                 __syncwarp();
                 st_shared_v4(words + lane * 16, v[0], v[1], v[2], v[3]);
+                if constexpr (!kSplit) {                                     // the same for the scale words of A (the splitting warps write theirs in place)
+                    const uint32_t own = base + S::kOffSfb + stage * 512;
+                    #pragma unroll
+                    for (uint32_t c = 0; c < 4; ++c) v[c] = c * 32 < kCols ? ld_shared_u32(own + (c * 32 + lane) * 4) : 0u;
+                    __syncwarp();
+                    st_shared_v4(own + lane * 16, v[0], v[1], v[2], v[3]);
+                }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full_bar(stage));
             }
-        } else if (warp >= 4) {
+        } else if (kSplit && warp >= 4) {
             const int rows = min(kTokens, end - r0), blocks = kb1 - kb0;
             const int team = (warp - 4) / S::kTeam, member = (warp - 4) % S::kTeam;
             // Piece i of this lane: elements 8 (lane % 16) .. of the K-block, of row 2 (i kTeam + member) + lane / 16
@@ -263,7 +309,7 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
             }
             steps += blocks;
         }
-        if (warp >= 4 && warp < 8) {
+        if (warp >= 4) {
             const int rows = min(kTokens, end - r0);
             // Epilogue: this thread's column of D, rows r0 .. r0 + rows
             const uint32_t quarter = warp % 4, row = quarter * 32 + lane;
@@ -287,6 +333,7 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
             const uint32_t own_rows = S::recv_rows(slices), recv = base + S::kOffRecv;
             __syncwarp();
             if (slices > 1) cluster_wait();                                  // every CTA of the cluster may be written to
+            uint32_t owner = 0, at_owner = 0;                                // row t of D: CTA t mod slices, its (t / slices)-th
             #pragma unroll
             for (int t0 = 0; t0 < kTokens; t0 += 16) {
                 uint32_t v[16], w[16];
@@ -300,8 +347,15 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                 for (int i = 0; i < (kTokens < 16 ? kTokens : 16); ++i) {
                     const int t = t0 + i;
                     const float y = !some ? 0.0f : __uint_as_float(v[i]) + __uint_as_float(kTokens >= 16 ? w[i] : v[i + 8]);
-                    if (slices == 1) write(t, y);
-                    else if (t < rows) st_shared_cluster_u32(map_to_cta(recv + ((rank * own_rows + t / slices) * 128 + row) * 4, t % slices), __float_as_uint(y));
+                    if (slices == 1) {
+                        write(t, y);
+                    } else if (t < rows) {
+                        st_shared_cluster_u32(map_to_cta(recv + ((rank * own_rows + at_owner) * 128 + row) * 4, owner), __float_as_uint(y));
+                        if (++owner == slices) {
+                            owner = 0;
+                            ++at_owner;
+                        }
+                    }
                 }
             }
             tc_fence_before_sync();
@@ -314,14 +368,18 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                 for (uint32_t i = 0; i < own_rows; ++i) {
                     const int t = static_cast<int>(i * slices + rank);
                     if (t >= rows) break;
-                    float y = 0.0f;
-                    for (uint32_t s = 0; s < slices; ++s) y += __uint_as_float(ld_shared_u32(recv + ((s * own_rows + i) * 128 + row) * 4));
+                    float part[kMaxCluster], y = 0.0f;                       // (all loads on their way before the first sum)
+                    #pragma unroll
+                    for (uint32_t s = 0; s < kMaxCluster; ++s)
+                        part[s] = s < slices ? __uint_as_float(ld_shared_u32(recv + ((s * own_rows + i) * 128 + row) * 4)) : 0.0f;
+                    #pragma unroll
+                    for (uint32_t s = 0; s < kMaxCluster; ++s) y += part[s];
                     write(t, y);
                 }
             }
         }
-        if (slices > 1 && (warp < 4 || warp >= 8)) {
-            // the other warps only take part in the two barriers of the epilogue
+        if (slices > 1 && warp < 4) {
+            // the role warps only take part in the two barriers of the epilogue
             __syncwarp();
             cluster_wait();
             cluster_arrive();

@@ -15,26 +15,132 @@
 namespace dg {
 namespace {
 
-// CTAs along K (a cluster) of a launch with `tiles` CTAs of 128 columns: enough to occupy the GPU, as long as each keeps four K-blocks
+// CTAs along K (a cluster) of a launch with `tiles` CTAs of 128 columns.  What a choice costs: the waves it takes (clusters live inside one
+// GPC, so fewer fit than SMs / size), times a CTA's K-blocks at ~0.2 us and ~3 us to start and end, a little more with partners.
+// (Clusters at once: what a 148-SM B200 reported for one CTA per SM; 32 clusters of 8 where 30 fit took twice the time of 6.)
 int choose_slices(int64_t tiles, int ctas_per_sm, int num_blocks) {
-    const int64_t slots = static_cast<int64_t>(dg_get_num_sms()) * ctas_per_sm;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({few::kMaxCluster, slots / tiles, num_blocks / 4})));
+    static const int kFit[few::kMaxCluster + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+    int best = 1;
+    double best_cost = 0.0;
+    for (int s = 1; s <= few::kMaxCluster && (s == 1 || num_blocks / s >= 2); ++s) {
+        const int64_t at_once = std::max<int64_t>(1, static_cast<int64_t>(kFit[s]) * ctas_per_sm * dg_get_num_sms() / 148);
+        const double cost = static_cast<double>(ceil_div(tiles, at_once)) * (0.2 * ceil_div(num_blocks, s) + 3.0 + (s > 1 ? 0.3 : 0.0));
+        if (s == 1 || cost < best_cost) {
+            best = s;
+            best_cost = cost;
+        }
+    }
+    return best;
 }
 
-template <int kTokens>
-int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p) {
-    using S = few::Shape<kTokens>;
+// A split ahead of the product: [hi, lo][slot][k] E4M3 bytes, then their scale words [k / 128][hi, lo][slot] (four UE8M0 codes, one per 32
+// elements of K).  A dense product's slots are its rows.
+struct Planes {
+    uint8_t* q;
+    uint32_t* sf;
+    int slots;
+};
+int num_slots(int m, int groups, bool ragged) { return align_up(ragged ? m + 4 * groups + 4 : m, 4); }
+size_t planes_bytes(int slots, int k) { return static_cast<size_t>(2) * slots * (k + k / 32); }
+
+constexpr int kSplitRows = 16, kSplitCols = 512;
+
+// One CTA splits 16 rows x 512 columns: 16-byte loads, quads of lanes share a scale, 8-byte stores, and the scale words of the 16 rows leave
+// together (they are neighbours when the rows are).  Bound by memory: 2 bytes in, 2 + 1/16 out per element.
+__global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* __restrict__ a, int64_t lda, const Planes out, int m, int k,
+                                                         const int* __restrict__ group_ends, int groups) {
+    __shared__ int slot_of[kSplitRows];
+    __shared__ uint32_t words[2][kSplitCols / 128][kSplitRows];
+    griddep_launch_dependents();
+    const int row0 = blockIdx.y * kSplitRows, r = threadIdx.x / 16, chunk = threadIdx.x % 16, row = row0 + r;
+    if (threadIdx.x < kSplitRows) {
+        const int mine = row0 + threadIdx.x;
+        int slot = mine < m ? mine : -1;
+        if (group_ends != nullptr && slot >= 0) {
+            // the group that holds the row: the first whose end lies behind it
+            int lo = 0, hi = groups;
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (group_ends[mid] > mine) hi = mid;
+                else lo = mid + 1;
+            }
+            const int first = lo == 0 ? 0 : min(max(group_ends[lo - 1], 0), m);
+            slot = lo == groups ? -1 : first_slot(first, lo) + mine - first;
+        }
+        slot_of[threadIdx.x] = slot;
+    }
+    __syncthreads();
+    const int slot = slot_of[r];
+    uint4 raw[kSplitCols / 128];
+    #pragma unroll
+    for (int b = 0; b < kSplitCols / 128; ++b) {
+        const int col = blockIdx.x * kSplitCols + b * 128 + chunk * 8;
+        raw[b] = make_uint4(0, 0, 0, 0);
+        if (slot >= 0 && col < k) raw[b] = __ldg(reinterpret_cast<const uint4*>(a + row * lda + col));
+    }
+    #pragma unroll
+    for (int b = 0; b < kSplitCols / 128; ++b) {
+        const int col = blockIdx.x * kSplitCols + b * 128 + chunk * 8;
+        uint2 hi, lo;
+        const uint32_t code = split_bf16(raw[b], hi, lo);
+        if (slot >= 0 && col < k) {
+            *reinterpret_cast<uint2*>(out.q + static_cast<int64_t>(slot) * k + col) = hi;
+            *reinterpret_cast<uint2*>(out.q + (static_cast<int64_t>(out.slots) + slot) * k + col) = lo;
+        }
+        uint32_t word = code << (chunk / 4 * 8);
+        word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
+        word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
+        if (chunk == 0) {
+            words[0][b][r] = word;
+            uint32_t less = 0;                                               // lo's codes: 4 less, NaN stays
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t c = word >> (8 * j) & 0xFFu;
+                less |= (c == 255u ? 255u : c - 4u) << (8 * j);
+            }
+            words[1][b][r] = less;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 2 * (kSplitCols / 128) * kSplitRows) {
+        const int i = threadIdx.x, rr = i % kSplitRows, b = i / kSplitRows % (kSplitCols / 128), plane = i / kSplitRows / (kSplitCols / 128);
+        const int kb = blockIdx.x * (kSplitCols / 128) + b;
+        if (slot_of[rr] >= 0 && kb < k / 128)
+            out.sf[(static_cast<int64_t>(kb) * 2 + plane) * out.slots + slot_of[rr]] = words[plane][b][rr];
+    }
+}
+
+int split_rows(const dg_gemm_args_t* g, const int* group_ends, const Planes& planes) {
+    const dim3 grid(ceil_div(g->k, kSplitCols), ceil_div(g->m, kSplitRows));
+    split_rows_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(g->stream)>>>(static_cast<const __nv_bfloat16*>(g->a), g->lda, planes, g->m, g->k, group_ends,
+                                                                               g->num_groups);
+    DG_CUDA_RT(cudaGetLastError());
+    return DG_OK;
+}
+
+template <int kTokens, bool kSplit>
+int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Planes& planes) {
+    using S = few::Shape<kTokens, kSplit>;
     const int tiles_n = ceil_div(g->n, 128), passes = p.group_ends != nullptr ? 1 : ceil_div(g->m, kTokens);
     const int slices = choose_slices(static_cast<int64_t>(tiles_n) * passes * g->num_groups, S::kCtasPerSm, g->k / 128);
-    CUtensorMap tm_w, tm_sf, tm_a;
+    CUtensorMap tm_w, tm_sf, tm_a, tm_sfa;
     int rc;
     const uint64_t words = ceil_div(g->k, 4 * g->gran_k_b);
     if ((rc = encode_tensor_map_2d(&tm_w, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, g->b, g->k, static_cast<uint64_t>(g->num_groups) * g->n, g->ldb, 128, 128,
                                    CU_TENSOR_MAP_SWIZZLE_128B)) != DG_OK) return rc;
     if ((rc = encode_tensor_map_2d(&tm_sf, CU_TENSOR_MAP_DATA_TYPE_INT32, g->sfb, g->n, words * g->num_groups, g->sfb_pitch * 4, 128, 1,
                                    CU_TENSOR_MAP_SWIZZLE_NONE)) != DG_OK) return rc;
-    if ((rc = encode_tensor_map_2d(&tm_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g->a, g->k, g->m, g->lda * 2, 128, kTokens, CU_TENSOR_MAP_SWIZZLE_NONE)) != DG_OK) return rc;
-    const auto kernel = few::bf16_fp4_few_rows_kernel<kTokens>;
+    if constexpr (kSplit) {
+        if ((rc = encode_tensor_map_2d(&tm_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g->a, g->k, g->m, g->lda * 2, 128, kTokens, CU_TENSOR_MAP_SWIZZLE_NONE)) != DG_OK) return rc;
+        tm_sfa = tm_a;                           // (not used)
+    } else {
+        if ((rc = encode_tensor_map_2d(&tm_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, planes.q, g->k, static_cast<uint64_t>(2) * planes.slots, g->k, 128, kTokens,
+                                       CU_TENSOR_MAP_SWIZZLE_128B)) != DG_OK) return rc;
+        if ((rc = encode_tensor_map_2d(&tm_sfa, CU_TENSOR_MAP_DATA_TYPE_INT32, planes.sf, planes.slots, static_cast<uint64_t>(2) * (g->k / 128),
+                                       static_cast<uint64_t>(planes.slots) * 4, kTokens, 2, CU_TENSOR_MAP_SWIZZLE_NONE)) != DG_OK) return rc;
+        if ((rc = split_rows(g, p.group_ends, planes)) != DG_OK) return rc;
+    }
+    const auto kernel = few::bf16_fp4_few_rows_kernel<kTokens, kSplit>;
     const int smem = S::smem_bytes(slices);
     DG_CUDA_RT(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg{};
@@ -49,16 +155,24 @@ int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p) {
         attrs[cfg.numAttrs].val.clusterDim.y = attrs[cfg.numAttrs].val.clusterDim.z = 1;
         ++cfg.numAttrs;
     }
-    if (state().pdl) {
+    if (state().pdl || !kSplit) {                // behind the kernel that splits A always: it lets this one start early
         attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
     cfg.attrs = attrs;
-    DG_CUDA_RT(cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_sf, tm_a, p));
+    DG_CUDA_RT(cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_sf, tm_a, tm_sfa, p));
     return DG_OK;
 }
 
-int run(const dg_gemm_args_t* g, bool ragged) {
+// Rows of A one product multiplies with a matrix of weights (ragged: on average; the sizes are on the device)
+int typical_rows(const dg_gemm_args_t* g, bool ragged) { return ragged ? ceil_div(g->m, g->num_groups) : g->m; }
+bool splits_inside(const dg_gemm_args_t* g, bool ragged) { return typical_rows(g, ragged) <= 8; }
+
+size_t workspace_bytes(const dg_gemm_args_t* g, bool ragged) {
+    return g->m == 0 || g->n == 0 || splits_inside(g, ragged) ? 0 : planes_bytes(num_slots(g->m, g->num_groups, ragged), g->k);
+}
+
+int run(const dg_gemm_args_t* g, bool ragged, void* workspace, int64_t given_bytes) {
     DG_REQUIRE_ALIVE();
     DG_REQUIRE(g != nullptr);
     DG_REQUIRE(g->a_dtype == DG_BF16 && g->b_dtype == DG_FP4_E2M1_X2);
@@ -81,19 +195,27 @@ int run(const dg_gemm_args_t* g, bool ragged) {
     DG_REQUIRE(g->ldd >= g->n && (g->ldd * d_elem) % 16 == 0);
     DG_REQUIRE(g->sfb_pitch >= align_up<int64_t>(g->n, 4) && g->sfb_pitch % 4 == 0);
 
+    const size_t needed = workspace_bytes(g, ragged);
+    DG_REQUIRE(needed == 0 || (workspace != nullptr && aligned(workspace, 128) && given_bytes >= 0 && static_cast<size_t>(given_bytes) >= needed));
     int rc = ensure_status_word();
     if (rc != DG_OK) return rc;
-    const Bf16Fp4Params p{g->d, ragged ? g->grouped_layout : nullptr, state().status_device, g->m, g->n, g->k, g->gran_k_b,
-                          g->ldd, g->d_dtype == DG_FP32, g->accumulate != 0, g->has_alpha ? g->alpha : 1.0f};
-    const int rows = ragged ? ceil_div(g->m, g->num_groups) : g->m;
-    if (rows <= 8) return launch_few_rows<8>(g, p);
-    if (rows <= 16) return launch_few_rows<16>(g, p);
-    if (rows <= 32) return launch_few_rows<32>(g, p);
-    return launch_few_rows<64>(g, p);
+    const int slots = num_slots(g->m, g->num_groups, ragged), rows = typical_rows(g, ragged);
+    const Planes planes{static_cast<uint8_t*>(workspace), reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + static_cast<size_t>(2) * slots * g->k), slots};
+    const Bf16Fp4Params p{g->d, ragged ? g->grouped_layout : nullptr, state().status_device, g->m, g->n, g->k, g->gran_k_b, g->ldd, g->d_dtype == DG_FP32,
+                          g->accumulate != 0, g->has_alpha ? g->alpha : 1.0f, slots};
+    if (splits_inside(g, ragged)) return launch_few_rows<8, true>(g, p, planes);
+    if (rows <= 16) return launch_few_rows<16, false>(g, p, planes);
+    if (rows <= 32) return launch_few_rows<32, false>(g, p, planes);
+    return launch_few_rows<64, false>(g, p, planes);
 }
 
 }  // namespace
 }  // namespace dg
 
-extern "C" int dg_bf16_fp4_gemm(const dg_gemm_args_t* args) { return dg::run(args, false); }
-extern "C" int dg_m_grouped_bf16_fp4_gemm_ragged(const dg_gemm_args_t* args) { return dg::run(args, true); }
+extern "C" int64_t dg_bf16_fp4_workspace_bytes(const dg_gemm_args_t* args, int ragged) {
+    return args == nullptr || args->m < 0 || args->k < 0 || args->num_groups <= 0 ? -1 : static_cast<int64_t>(dg::workspace_bytes(args, ragged != 0));
+}
+extern "C" int dg_bf16_fp4_gemm(const dg_gemm_args_t* args, void* workspace, int64_t workspace_bytes) { return dg::run(args, false, workspace, workspace_bytes); }
+extern "C" int dg_m_grouped_bf16_fp4_gemm_ragged(const dg_gemm_args_t* args, void* workspace, int64_t workspace_bytes) {
+    return dg::run(args, true, workspace, workspace_bytes);
+}

@@ -9,6 +9,7 @@
 // families, settings).  The checks and their messages are the ones api.py applies to the same call.
 #include <torch/extension.h>
 
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <optional>
@@ -253,6 +254,63 @@ bool m_grouped_masked(const TensorPair& a_pair, const TensorPair& b_pair, const 
     return true;
 }
 
+// bf16_fp4_gemm_nt and m_grouped_bf16_fp4_gemm_nt_ragged with packed scales: one matrix of weights, or one per group and the ends
+// of the groups' rows.  Launches on the tensors' device, on its current stream.
+bool bf16_fp4(const torch::Tensor& a, const TensorPair& b_pair, const torch::Tensor& d, const std::optional<torch::Tensor>& c,
+              const std::optional<torch::Tensor>& group_ends, const py::object& recipe_b, std::optional<double> alpha) {
+    const torch::Tensor &w = b_pair.first, &sf = b_pair.second;
+    const bool ragged = group_ends.has_value();
+    if (sf.scalar_type() != torch::kInt || (c.has_value() && c->unsafeGetTensorImpl() != d.unsafeGetTensorImpl())) return false;
+    if (!PyTuple_Check(recipe_b.ptr()) || PyTuple_GET_SIZE(recipe_b.ptr()) != 2) return false;
+    const long gran_mn = PyLong_AsLong(PyTuple_GET_ITEM(recipe_b.ptr(), 0)), gran_k = PyLong_AsLong(PyTuple_GET_ITEM(recipe_b.ptr(), 1));
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    if (gran_mn != 1 || (gran_k != 32 && gran_k != 128)) return false;
+    DG_BIND_REQUIRE(a.dim() == 2 && w.dim() == (ragged ? 3 : 2) && d.dim() == 2, "t.dim() == N");
+    const int64_t m = a.size(0), k = a.size(1), n = w.size(-2), groups = ragged ? w.size(0) : 1;
+    DG_BIND_REQUIRE(m == d.size(0) && n == d.size(1) && k == 2 * w.size(-1), "m == m_ and n == n_ and k == k_");
+    DG_BIND_REQUIRE(d.scalar_type() == torch::kBFloat16 || (d.scalar_type() == torch::kFloat && !ragged), "d.scalar_type() == torch::kBFloat16");
+    if (ragged) {
+        DG_BIND_REQUIRE(n > 0 && k > 0 && groups > 0, "n > 0 and k > 0 and num_groups > 0");
+        DG_BIND_REQUIRE(w.stride(0) == n * w.stride(1), "the groups of b follow one another");
+        DG_BIND_REQUIRE(group_ends->is_cuda() && group_ends->get_device() == d.get_device() && group_ends->scalar_type() == torch::kInt &&
+                            group_ends->dim() == 1 && group_ends->is_contiguous() && group_ends->size(0) == groups,
+                        "group_ends: contiguous int32 [num_groups] on the device of d");
+    }
+    if (m == 0 || n == 0) return true;
+    if (k == 0) return false;                    // (zeroing or copying D is the general path's)
+    DG_BIND_REQUIRE(a.scalar_type() == torch::kBFloat16 && w.scalar_type() == kPackedFP4, "a: bfloat16, b: packed FP4 (int8)");
+    DG_BIND_REQUIRE(a.is_cuda() && w.is_cuda() && sf.is_cuda() && d.is_cuda() && a.get_device() == d.get_device() && w.get_device() == d.get_device() &&
+                        sf.get_device() == d.get_device(), "a, b, d are CUDA tensors of one device");
+    DG_BIND_REQUIRE(a.stride(1) == 1 && w.stride(-1) == 1, "major_a == cute::UMMA::Major::K and major_b == cute::UMMA::Major::K");
+    DG_BIND_REQUIRE(d.stride(1) == 1 || n == 1, "t.stride(-1) == 1");
+    check_packed_sf(sf, n, k, static_cast<int>(gran_k), ragged ? std::optional<int64_t>(groups) : std::nullopt);
+    const c10::cuda::OptionalCUDAGuard guard(d.device());
+    dg_gemm_args_t g{};
+    g.a = a.data_ptr(); g.b = w.data_ptr(); g.sfb = sf.data_ptr(); g.d = d.data_ptr();
+    g.m = static_cast<int32_t>(m); g.n = static_cast<int32_t>(n); g.k = static_cast<int32_t>(k); g.num_groups = static_cast<int32_t>(groups);
+    g.a_dtype = DG_BF16; g.b_dtype = DG_FP4_E2M1_X2;
+    g.d_dtype = d.scalar_type() == torch::kBFloat16 ? DG_BF16 : DG_FP32;
+    g.major_a = g.major_b = DG_MAJOR_K;
+    // (the pitch of a single row says nothing: torch may report any stride for it)
+    g.lda = m > 1 ? a.stride(0) : k; g.ldb = w.stride(-2); g.ldd = m > 1 ? d.stride(0) : align_up(n, 8);
+    g.sfb_pitch = sf.stride(-1); g.gran_k_b = static_cast<int32_t>(gran_k);
+    g.accumulate = c.has_value() ? 1 : 0;
+    g.has_alpha = alpha.has_value() ? 1 : 0;
+    g.alpha = alpha.has_value() ? static_cast<float>(*alpha) : 1.0f;
+    g.grouped_layout = ragged ? group_ends->data_ptr<int32_t>() : nullptr;
+    g.stream = c10::cuda::getCurrentCUDAStream(d.get_device()).stream();
+    const int64_t bytes = dg_bf16_fp4_workspace_bytes(&g, ragged ? 1 : 0);
+    // the call's own: the allocator hands it to another stream, or a captured graph's pool to another graph, only with the order kept
+    torch::Tensor workspace;
+    if (bytes > 0) workspace = at::empty({bytes}, d.options().dtype(torch::kUInt8));
+    void* const ws = bytes > 0 ? workspace.data_ptr() : nullptr;
+    check_rc(ragged ? dg_m_grouped_bf16_fp4_gemm_ragged(&g, ws, bytes) : dg_bf16_fp4_gemm(&g, ws, bytes));
+    return true;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_C, m) {
@@ -260,4 +318,5 @@ PYBIND11_MODULE(_C, m) {
     m.def("dense_nt", &dense_nt);
     m.def("m_grouped_contiguous", &m_grouped_contiguous);
     m.def("m_grouped_masked", &m_grouped_masked);
+    m.def("bf16_fp4", &bf16_fp4);
 }

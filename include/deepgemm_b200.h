@@ -226,9 +226,13 @@ DG_API int dg_fp8_bmm(const dg_gemm_args_t* args);
  * ragged: grouped_layout = int32[num_groups] on the device, the row where each group ends; group g is the rows
  * [grouped_layout[g - 1], grouped_layout[g]) (from row 0 for g = 0) of A [m, k] and D [m, n], with no padding between
  * groups and no alignment; ends must not decrease; rows at or behind the last end are not written.
- * Sums are FP32, one rounding per element of D.  A row of A with an infinity or a NaN gives non-finite results. */
-DG_API int dg_bf16_fp4_gemm(const dg_gemm_args_t* args);
-DG_API int dg_m_grouped_bf16_fp4_gemm_ragged(const dg_gemm_args_t* args);
+ * Sums are FP32, one rounding per element of D.  A row of A with an infinity or a NaN gives non-finite results.
+ * workspace: device memory of this call alone until it has completed, 128-byte aligned, at least
+ * dg_bf16_fp4_workspace_bytes(args, ragged) bytes (0 up to eight rows per matrix of weights; about 2 m k above; reads only the
+ * sizes in args; -1: no valid sizes). */
+DG_API int64_t dg_bf16_fp4_workspace_bytes(const dg_gemm_args_t* args, int ragged);
+DG_API int dg_bf16_fp4_gemm(const dg_gemm_args_t* args, void* workspace_device, int64_t workspace_bytes);
+DG_API int dg_m_grouped_bf16_fp4_gemm_ragged(const dg_gemm_args_t* args, void* workspace_device, int64_t workspace_bytes);
 
 /* Same operation and arguments as dg_fp8_fp4_gemm, for callers that cannot allocate device memory at call time: a
  * serving thread that must never block on the allocator's locks, a process that hands out its whole memory budget at

@@ -27,22 +27,22 @@ REFUSED = [dict(a_dtype=_lib.DG_FP8_E4M3), dict(b_dtype=_lib.DG_BF16), dict(d_dt
 
 @pytest.mark.parametrize("kw", REFUSED + [dict(num_groups=2), dict(k=0)], ids=str)
 def test_dense_refuses(kw):
-    assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(**kw))) != _lib.DG_OK
+    assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(**kw)), None, 0) != _lib.DG_OK
     assert _lib.last_error()
 
 
 @pytest.mark.parametrize("kw", REFUSED + [dict(grouped_layout=None), dict(grouped_layout=0x6002), dict(num_groups=0), dict(num_groups=65536), dict(n=0), dict(k=0),
                                           dict(accumulate=1), dict(has_alpha=1), dict(d_dtype=_lib.DG_FP32)], ids=str)
 def test_ragged_refuses(kw):
-    assert _lib.lib.dg_m_grouped_bf16_fp4_gemm_ragged(C.byref(args(**{"num_groups": 3, "grouped_layout": 0x6000, **kw}))) != _lib.DG_OK
+    assert _lib.lib.dg_m_grouped_bf16_fp4_gemm_ragged(C.byref(args(**{"num_groups": 3, "grouped_layout": 0x6000, **kw})), None, 0) != _lib.DG_OK
     assert _lib.last_error()
 
 
 def test_null_arguments_and_empty_products():
     for fn in (_lib.lib.dg_bf16_fp4_gemm, _lib.lib.dg_m_grouped_bf16_fp4_gemm_ragged):
-        assert fn(None) != _lib.DG_OK
-    assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(m=0))) == _lib.DG_OK
-    assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(n=0))) == _lib.DG_OK
+        assert fn(None, None, 0) != _lib.DG_OK
+    assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(m=0)), None, 0) == _lib.DG_OK
+    assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(n=0)), None, 0) == _lib.DG_OK
 
 
 def test_python_functions_refuse_cpu_tensors_and_wrong_shapes():
@@ -56,3 +56,14 @@ def test_python_functions_refuse_cpu_tensors_and_wrong_shapes():
         dg.bf16_fp4_gemm_nt(a[0], (w, sf), d)
     with pytest.raises(RuntimeError, match="group_ends"):
         dg.m_grouped_bf16_fp4_gemm_nt_ragged(a, (w.expand(2, 64, 128).contiguous(), sf), d, torch.zeros(2, dtype=torch.int))
+
+
+def test_workspace():
+    size = lambda ragged=0, **kw: _lib.lib.dg_bf16_fp4_workspace_bytes(C.byref(args(**kw)), ragged)  # noqa: E731
+    assert size(m=8) == 0 and size(m=0) == 0 and size(m=24, num_groups=3, ragged=1) == 0
+    assert size(m=101) == 2 * 104 * (256 + 8)                                  # two planes of E4M3 and a scale per 32 of them, rows in fours
+    assert size(m=101, num_groups=3, ragged=1) >= 2 * (101 + 3 * 3) * (256 + 8)        # every group starts on a multiple of four
+    assert _lib.lib.dg_bf16_fp4_workspace_bytes(None, 0) == -1 and size(m=-1) == -1 and size(num_groups=0, ragged=1) == -1
+    for kw in (dict(workspace=None), dict(workspace=0x7000, given=100), dict(workspace=0x7040), dict(workspace=0x7000, given=-1)):
+        assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(m=64)), kw.get("workspace"), kw.get("given", 1 << 20)) != _lib.DG_OK
+        assert "workspace" in _lib.last_error()
