@@ -15,7 +15,7 @@ DG_OK = 0
 DG_FP8_E4M3, DG_FP4_E2M1_X2, DG_BF16, DG_FP32 = 0, 1, 2, 3
 DG_MAJOR_K, DG_MAJOR_MN = 0, 1
 DG_GEMM_DENSE, DG_GEMM_M_GROUPED_CONTIGUOUS, DG_GEMM_M_GROUPED_MASKED, DG_GEMM_M_GROUPED_CONTIGUOUS_PSUM = 0, 1, 2, 3
-DG_GEMM_K_GROUPED_CONTIGUOUS, DG_GEMM_BATCHED = 4, 5
+DG_GEMM_K_GROUPED_CONTIGUOUS, DG_GEMM_BATCHED, DG_GEMM_M_GROUPED_RAGGED = 4, 5, 6
 
 
 class GemmArgs(C.Structure):

@@ -27,13 +27,9 @@
 #include <cuda_fp16.h>
 
 #include "ptx.cuh"
+#include "tile_scheduler.cuh"
 
 namespace dg {
-
-// The rows of A split ahead of the product (dg_bf16_fp4.cu) lie in slots: those of group g from a multiple of four on, so that a TMA
-// copy of their scale words may start there.  Groups keep their order and do not overlap: the next one's first slot is behind the last row
-// of this one's, whatever its size.
-__host__ __device__ __forceinline__ int first_slot(int first_row, int group) { return (first_row + 3) / 4 * 4 + 4 * group; }
 
 struct Bf16Fp4Params {
     void* d;                     // [m, n], pitch ldd

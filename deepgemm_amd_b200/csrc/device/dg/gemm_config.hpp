@@ -32,6 +32,9 @@ struct GemmLayout {
                                                    // The MMA still reads 128 rows: the rest is whatever follows in shared
                                                    // memory and lands in accumulator rows that are never stored
 
+    uint32_t planes = 1;                           // 2: A is a BF16 matrix split into two E4M3 planes; a stage holds block_m rows of each, both
+                                                   // multiplied with the stage's B into one accumulator
+
     // A packed scale word covers 4 * gran_k elements of K: it is fetched on every `period`-th K-block of a work item,
     // into the next of a ring of buffers.  A buffer may be refilled once the fetch it held is no longer among the
     // last num_stages pipeline steps (the producer is never further ahead of the MMAs).  num_stages consecutive steps
@@ -71,12 +74,12 @@ struct GemmLayout {
     DG_HDC uint32_t num_store_stages() const { return store_buffers * (block_m / 128); }
 
     DG_HDC uint32_t a_stage_rows() const { return a_rows ? a_rows : block_m; }
-    DG_HDC uint32_t a_bytes() const { return a_stage_rows() * block_k; }  // one byte per element (FP8, or FP4 in 16-byte containers)
+    DG_HDC uint32_t a_bytes() const { return a_stage_rows() * block_k * planes; }  // one byte per element (FP8, or FP4 in 16-byte containers)
     DG_HDC uint32_t load_block_n() const { return block_n / cluster; }
     // MN-major only: atoms of [block_k / ab_elem_bytes rows of K][128 bytes of N]
     DG_HDC uint32_t b_atoms() const { return (load_block_n() * ab_elem_bytes + 127) / 128; }
     DG_HDC uint32_t b_bytes() const { return b_mn_major ? b_atoms() * 128 * (block_k / ab_elem_bytes) : load_block_n() * block_k; }
-    DG_HDC uint32_t sfa_bytes() const { return block_m * 4 * sfa_words(); }          // [word of K][row] int32
+    DG_HDC uint32_t sfa_bytes() const { return block_m * 4 * sfa_words() * planes; }          // [word of K][row] int32 ([plane][row] with two planes)
     DG_HDC uint32_t sfb_bytes() const { return sf_block_n() * 4 * sfb_words(); }
 
     DG_HDC uint32_t off_d() const { return 0; }
@@ -98,7 +101,7 @@ struct GemmLayout {
     // halves of one tile when it is 256), then SFA (4 columns per 128 rows) and SFB (4 columns per 128 columns of the tile)
     DG_HDC uint32_t tmem_col_sfa() const { return 2 * block_n; }
     // (per packed word of a stage: kind::mxf4 stages hold two)
-    DG_HDC uint32_t tmem_col_sfb() const { return tmem_col_sfa() + block_m / 32 * sfa_words(); }
+    DG_HDC uint32_t tmem_col_sfb() const { return tmem_col_sfa() + block_m / 32 * sfa_words() * planes; }
     DG_HDC uint32_t tmem_cols_used() const { return ab_elem_bytes != 1 ? 2 * block_n : tmem_col_sfb() + sf_block_n() / 32 * sfb_words(); }
     DG_HDC uint32_t tmem_cols_alloc() const {
         const uint32_t u = tmem_cols_used();

@@ -43,6 +43,12 @@
 // 128 bytes, now 64 elements of K; the MMA is tcgen05.mma.kind::f16 (16 elements of K per instruction); the scale loads,
 // the rearranging warp's work and the scale columns of tensor memory disappear; MN-major atoms are 64 elements wide.
 //
+// DG_PLANES == 2: A is a BF16 matrix split into two E4M3 matrices, A = hi + lo with a scale per 32 elements of K each (dg_bf16_fp4.cu), and
+// the product is hi B^T + lo B^T: a stage holds 128 rows of either and one B, which both MMAs of a K-block read into one accumulator.  Two
+// E4M3 x E2M1 MMAs take the time of one in BF16, without B ever being widened.
+//
+// ragged (type 6): groups of rows of any size follow one another in D without padding; the rows of A lie in slots (tile_scheduler.cuh).
+//
 // DG_SPLIT_K (dense only, for shapes with too few output tiles to fill the GPU): every output tile becomes
 // num_splits work items over slices of K, and the kernel's D is an FP32 workspace of num_splits stacked
 // [rows x N] panels: work item (tile, slice) stores its partial tile into panel `slice`.  A separate kernel
@@ -138,6 +144,10 @@ constexpr uint32_t kSplitCluster = DG_SPLIT_CLUSTER;   // CTAs of a cluster shar
 
 constexpr uint32_t kMHalves    = DG_M_HALVES;      // 128-row MMAs per CTA and K-block (1 or 2)
 constexpr uint32_t kL2Hint     = DG_L2_HINT;
+#ifndef DG_PLANES
+#define DG_PLANES 1
+#endif
+constexpr uint32_t kPlanes     = DG_PLANES;        // E4M3 matrices that make up A
 
 constexpr uint32_t UMMA_M = 128 * kCluster, UMMA_N = BLOCK_N, UMMA_K = 32;
 constexpr uint32_t LOAD_BLOCK_N = BLOCK_N / kCluster;      // rows of B each CTA loads
@@ -224,9 +234,13 @@ static_assert(kSplitCluster == 1 || (kGemmType == kDense && !kSplitK && kCluster
 #define DG_A_ROWS 0
 #endif
 constexpr GemmLayout kLayout{CTA_M, BLOCK_N, BLOCK_K, kNumStages, kDElemBytes, kCluster, kBMnMajor ? 1u : 0u, kGranKA, kGranKB,
-                             DG_SHORT_K, kABElemBytes, DG_STORE_BUFFERS, kMXF4 ? 1u : 0u, DG_A_ROWS};
+                             DG_SHORT_K, kABElemBytes, DG_STORE_BUFFERS, kMXF4 ? 1u : 0u, DG_A_ROWS, kPlanes};
 static_assert(DG_A_ROWS == 0 || (DG_A_ROWS % 8 == 0 && DG_A_ROWS < 128 && kGemmType == kDense && kCluster == 1 && kMHalves == 1 && !kAMnMajor),
               "a shortened A stage: dense GEMMs with fewer rows than one tile, K-major A, one CTA per tile");
+static_assert(kPlanes == 1 || (kPlanes == 2 && kMHalves == 1 && kHasSF && !kMXF4 && !kAIsFP4 && !kAMnMajor && !kBMnMajor && BLOCK_K == 128 && kGranKA == 32 &&
+                               DG_A_ROWS == 0 && !kTransposedD && (kGemmType == kDense || kGemmType == kMGroupedRagged)),
+              "split A: K-major E4M3 planes with one scale per 32 elements, 128 rows per CTA, dense and ragged");
+static_assert(kGemmType != kMGroupedRagged || (kPlanes == 2 && kCluster == 1), "ragged groups: built for a split A, one CTA per tile");
 constexpr uint32_t kSFAWords = kHasSF ? kLayout.sfa_words() : 1, kSFBWords = kHasSF ? kLayout.sfb_words() : 1;   // packed words per row and stage
 // K coordinate of a K-major load advances by this much per K-block: elements of the tensor map's type (bytes for the
 // packed operands of kind::mxf4, whose maps are plain byte maps)
@@ -296,6 +310,7 @@ struct GemmParams {
     uint32_t* sfd;               // quantising epilogue: packed UE8M0 scales of D, word (row, column / 128) at sfd[(column / 128) * sfd_pitch + row]
     uint32_t sfd_pitch;
     uint32_t kb_per_batch;       // batch-reduced GEMM: K-blocks in one batch
+    uint32_t plane_rows;         // split A: rows between the two planes
 };
 
 // Wait-time accounting for tuning: with DG_PROFILE defined every role adds the cycles it spent inside each
@@ -531,7 +546,8 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                             if (kb % kSFBPeriod == 0) sf_bytes += kSFBBytes;
                             mbar_arrive_expect_tx(sf_full_bar(stage), sf_bytes);
                             if (kb % kSFAPeriod == 0)
-                                tma_in(sfa_buffer(), &tm_sfa, sf_full_bar(stage), sfa_mn, sfa_row0 + kb / kSFAPeriod * kSFAWords, tile.group);
+                                // (split A: the two planes' words of a K-block are two rows, one box)
+                                tma_in(sfa_buffer(), &tm_sfa, sf_full_bar(stage), sfa_mn, sfa_row0 + kb / kSFAPeriod * kSFAWords * kPlanes, tile.group);
                             if (kb % kSFBPeriod == 0)
                                 tma_in(sfb_buffer(), &tm_sfb, sf_full_bar(stage), tile.n_block * BLOCK_N, sfb_row0 + kb / kSFBPeriod * kSFBWords, tile.group);
                         }
@@ -566,6 +582,8 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                             #pragma unroll
                             for (uint32_t ka = 0; ka < kKAtoms; ++ka)       // one box of the stage's rows per 128 bytes of K
                                 load(smem_base + kSmemA + stage * kABytes + ka * kAAtomStride, &tm_a, k_base + kb * kLoadXPerKBlock + ka * 128, a_row);
+                            if constexpr (kPlanes == 2)
+                                load(smem_base + kSmemA + stage * kABytes + kABytes / 2, &tm_a, k_base + kb * kLoadXPerKBlock, p.plane_rows + a_row);
                         } else {
                             // one box per atom: 128 bytes of M (128 FP8 or 64 BF16 elements) by the stage's rows of K
                             #pragma unroll
@@ -660,7 +678,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                         DG_PROF_FINE_BEGIN(prof_i0);
                         if (kHasSF && kb % kSFAPeriod == 0) {
                             #pragma unroll
-                            for (uint32_t i = 0; i < kSFAWords * SF_BLOCK_M / 128; ++i)      // chunk (word w, rows 128 r ..): index w * (rows / 128) + r
+                            for (uint32_t i = 0; i < kSFAWords * SF_BLOCK_M / 128 * kPlanes; ++i)      // chunk (word w, rows 128 r ..): index w * (rows / 128) + r
                                 tc_cp_32x128b_warpx4<kCluster>(tmem_base + kTmemColSFA + i * 4,
                                                                make_smem_desc(sfa_buffer() + i * 512, 0, 128, kSwizzleNone));
                         }
@@ -674,6 +692,8 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                         DG_PROF_FINE_BEGIN(prof_i1);
                         const uint64_t a_desc = make_smem_desc(smem_base + kSmemA + stage * kABytes, kALbo, kASbo, kASwizzle);
                         const uint64_t b_desc = make_smem_desc(smem_base + kSmemB + stage * kBBytes, kBLbo, kBSbo, kBSwizzle);
+                        #pragma unroll
+                        for (uint32_t pl = 0; pl < kPlanes; ++pl)
                         #pragma unroll
                         for (uint32_t h = 0; h < kMHalves; ++h) {
                             // In a two-pass tile (halves of different experts) pass p carries half p's expert
@@ -697,9 +717,9 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                                                           tmem_base + kTmemColSFA + (j / 2) * (SF_BLOCK_M / 32) + h * 4,
                                                           tmem_base + kTmemColSFB + (j / 2) * (SF_BLOCK_N / 32), ((kb - kb0) | j) != 0);
                                 else
-                                    tc_mma_mxf8f6f4<kCluster>(tmem_d, a_desc + h * ((BLOCK_M * BLOCK_K) >> 4) + a_step(j), b_desc + b_step(j),
+                                    tc_mma_mxf8f6f4<kCluster>(tmem_d, a_desc + (h + pl) * ((BLOCK_M * BLOCK_K) >> 4) + a_step(j), b_desc + b_step(j),
                                                               instr_desc_with_sf_ids(idesc, sfa_id, sfb_id),
-                                                              tmem_base + kTmemColSFA + h * 4, tmem_base + kTmemColSFB, ((kb - kb0) | j) != 0);
+                                                              tmem_base + kTmemColSFA + (h + pl) * 4, tmem_base + kTmemColSFB, ((kb - kb0) | j | pl) != 0);
                             }
                         }
                         DG_PROF_FINE_ADD(prof_mma, prof_i1);
@@ -754,7 +774,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                     DG_PROF_ADD(prof_wait, prof_w);
                     if (kb % kSFAPeriod == 0) {
                         #pragma unroll
-                        for (uint32_t i = 0; i < kSFAWords * SF_BLOCK_M / 128; ++i)
+                        for (uint32_t i = 0; i < kSFAWords * SF_BLOCK_M / 128 * kPlanes; ++i)
                             rearrange(sfa_buffer() + i * 512);
                     }
                     if (kb % kSFBPeriod == 0) {
@@ -991,7 +1011,8 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
             const uint32_t valid_rows = tile.valid_rows <= rows_before ? 0u :
                                         (tile.valid_rows - rows_before < BLOCK_M ? tile.valid_rows - rows_before : BLOCK_M);
             // (fewer than 128 only in a ragged tile of the masked and prefix-sum layouts: those rows are stored one by one)
-            const bool direct = (kGemmType == kMGroupedMasked || kGemmType == kMGroupedPsum || kGemmType == kKGrouped) && valid_rows < BLOCK_M;
+            const bool direct = (kGemmType == kMGroupedMasked || kGemmType == kMGroupedPsum || kGemmType == kKGrouped || kGemmType == kMGroupedRagged) &&
+                                valid_rows < BLOCK_M;
             auto release_tmem = [&]() {
                 tc_fence_before_sync();
                 if (kCluster == 1 || is_leader) mbar_arrive(tmem_empty_bar(accum));

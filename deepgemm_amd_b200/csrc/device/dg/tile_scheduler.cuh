@@ -20,6 +20,8 @@
 //       K-blocks and the first packed scale row of the group.  layout[g] is the slice's length (a multiple
 //       of the alignment) or, in the prefix-sum form, the element where it ends, the next slice starting
 //       at the following multiple of the alignment (scheduler/gemm.cuh:226-250 of the reference).
+//   m-grouped ragged : layout[g] is the row of D where group g ends and group g + 1 starts, no padding between them; the rows of A lie in
+//       slots, the groups' first ones on multiples of four (first_slot).  Walked on the device like the masked layout.
 //   batched : num_groups independent GEMMs of one shape; tile_id = batch * tiles_per_batch + tile, the
 //       batch being the third tensor-map coordinate of every operand (scheduler/gemm.cuh:251-263).
 #pragma once
@@ -34,7 +36,12 @@
 
 namespace dg {
 
-enum GemmKind : uint32_t { kDense = 0, kMGroupedContiguous = 1, kMGroupedMasked = 2, kMGroupedPsum = 3, kKGrouped = 4, kBatched = 5 };
+enum GemmKind : uint32_t { kDense = 0, kMGroupedContiguous = 1, kMGroupedMasked = 2, kMGroupedPsum = 3, kKGrouped = 4, kBatched = 5, kMGroupedRagged = 6 };
+
+// The rows of A of a ragged grouped GEMM lie in slots: those of group g from a multiple of four on, so that a TMA copy of their scale words
+// may start there.  Groups keep their order and do not overlap: the next one's first slot is behind the last row of this one's, whatever
+// its size.
+DG_HD int first_slot(int first_row, int group) { return (first_row + 3) / 4 * 4 + 4 * group; }
 
 struct Tile {
     uint32_t m_block;       // row block inside the group (masked) or inside A (dense / contiguous)
@@ -184,6 +191,29 @@ struct TileScheduler {
             t.a_row_base = t.d_row_base = t.sfa_mn_base = group_start;
             t.sfa_group = 0;
             const uint32_t left = rows - t.m_block * kBlockM;            // (rows already reach the aligned end when the padding is written)
+            t.valid_rows = left < kBlockM ? left : kBlockM;
+            t.split = 0;
+            t.mn_index = tile_id;
+            return true;
+        } else if constexpr (kKind == kMGroupedRagged) {
+            uint32_t mb = 0, rows = 0;
+            while (true) {
+                if (cur_group >= num_groups) return false;
+                const int e = layout[cur_group];
+                uint32_t end = e < 0 ? 0u : (static_cast<uint32_t>(e) > shape_m ? shape_m : static_cast<uint32_t>(e));
+                rows = end > group_start ? end - group_start : 0u;
+                mb = (rows + kBlockM - 1) / kBlockM;
+                if (tile_id < group_first_tile + mb * num_n_blocks) break;
+                group_first_tile += mb * num_n_blocks;
+                group_start = end;
+                ++cur_group;
+            }
+            rasterise(tile_id - group_first_tile, mb, t.m_block, t.n_block);
+            t.group = t.group1 = cur_group;
+            t.a_row_base = t.sfa_mn_base = static_cast<uint32_t>(first_slot(static_cast<int>(group_start), static_cast<int>(cur_group)));
+            t.d_row_base = group_start;
+            t.sfa_group = 0;
+            const uint32_t left = rows - t.m_block * kBlockM;
             t.valid_rows = left < kBlockM ? left : kBlockM;
             t.split = 0;
             t.mn_index = tile_id;

@@ -13,6 +13,9 @@
 #include "device/dg/bf16_fp4_few_rows.cuh"
 
 namespace dg {
+
+int run_split_a_gemm(const dg_gemm_args_t* args, bool ragged, int plane_rows);       // dg_gemm.cpp
+
 namespace {
 
 // CTAs along K (a cluster) of a launch with `tiles` CTAs of 128 columns.  What a choice costs: the waves it takes (clusters live inside one
@@ -164,6 +167,20 @@ int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Plane
     return DG_OK;
 }
 
+// The GEMM kernel on the two planes (its tiles are 128 rows of A; the form above has 128 columns of D and as many rows as there are)
+int launch_many_rows(const dg_gemm_args_t* g, bool ragged, const Planes& planes) {
+    int rc = split_rows(g, ragged ? g->grouped_layout : nullptr, planes);
+    if (rc != DG_OK) return rc;
+    dg_gemm_args_t args = *g;
+    args.a = planes.q;
+    args.sfa = planes.sf;
+    args.a_dtype = DG_FP8_E4M3;
+    args.lda = g->k;
+    args.gran_k_a = 32;
+    args.sfa_pitch = planes.slots;
+    return run_split_a_gemm(&args, ragged, planes.slots);
+}
+
 // Rows of A one product multiplies with a matrix of weights (ragged: on average; the sizes are on the device)
 int typical_rows(const dg_gemm_args_t* g, bool ragged) { return ragged ? ceil_div(g->m, g->num_groups) : g->m; }
 bool splits_inside(const dg_gemm_args_t* g, bool ragged) { return typical_rows(g, ragged) <= 8; }
@@ -205,8 +222,9 @@ int run(const dg_gemm_args_t* g, bool ragged, void* workspace, int64_t given_byt
                           g->accumulate != 0, g->has_alpha ? g->alpha : 1.0f, slots};
     if (splits_inside(g, ragged)) return launch_few_rows<8, true>(g, p, planes);
     if (rows <= 16) return launch_few_rows<16, false>(g, p, planes);
-    if (rows <= 32) return launch_few_rows<32, false>(g, p, planes);
-    return launch_few_rows<64, false>(g, p, planes);
+    // (the GEMM kernel stores whole 16-byte pieces of a row of D: where N ends inside one, what follows the row would not stay)
+    if (rows <= 32 || (static_cast<int64_t>(g->n) * d_elem) % 16 != 0) return launch_few_rows<32, false>(g, p, planes);
+    return launch_many_rows(g, ragged, planes);
 }
 
 }  // namespace

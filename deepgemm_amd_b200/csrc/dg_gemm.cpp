@@ -35,6 +35,7 @@ struct GemmParams {
     uint32_t* sfd;
     uint32_t sfd_pitch;
     uint32_t kb_per_batch;
+    uint32_t plane_rows;
 };
 
 // Split-K scratch: num_splits stacked FP32 [rows x N] panels.  One buffer per device, shared by every stream (a
@@ -79,12 +80,13 @@ struct Problem {
     bool k_psum;             // k-grouped: grouped_layout holds prefix sums
     bool stochastic;         // BF16 output rounded stochastically
     int reduce_batches;      // dense BF16 GEMM summed over this many batches as well (k is then batches x K of one batch); 0 = no
+    int planes;              // 2: A is a BF16 matrix split into two E4M3 planes (dense and ragged)
     bool mxf4;               // FP4 x FP4 through kind::mxf4 (packed operands in shared memory, 256 elements of K per stage)
 };
 
 int validate(int kind, const dg_gemm_args_t* a, bool need_pointers, Problem* p) {
     DG_REQUIRE(a != nullptr);
-    DG_REQUIRE(kind == DG_GEMM_DENSE || kind == DG_GEMM_M_GROUPED_CONTIGUOUS || kind == DG_GEMM_M_GROUPED_MASKED ||
+    DG_REQUIRE(kind == DG_GEMM_DENSE || kind == DG_GEMM_M_GROUPED_CONTIGUOUS || kind == DG_GEMM_M_GROUPED_MASKED || kind == DG_GEMM_M_GROUPED_RAGGED ||
                kind == DG_GEMM_M_GROUPED_CONTIGUOUS_PSUM || kind == DG_GEMM_K_GROUPED_CONTIGUOUS || kind == DG_GEMM_BATCHED);
     const bool k_grouped = kind == DG_GEMM_K_GROUPED_CONTIGUOUS, batched = kind == DG_GEMM_BATCHED;
     // BF16 operands (no scales): the reference's bf16_gemm_* family, same kernel with the scale path compiled out
@@ -156,6 +158,7 @@ int validate(int kind, const dg_gemm_args_t* a, bool need_pointers, Problem* p) 
         p->reduce_batches = a->reduce_batches;
     }
     p->kind = kind;
+    p->planes = 1;
     p->a_mn_major = a->major_a == DG_MAJOR_MN;
     p->b_mn_major = a->major_b == DG_MAJOR_MN;
     p->m = a->m; p->n = a->n; p->k = a->k * std::max(1, p->reduce_batches); p->groups = a->num_groups;
@@ -233,6 +236,7 @@ int validate(int kind, const dg_gemm_args_t* a, bool need_pointers, Problem* p) 
 // whole number of pair tiles (alignment 256 or 512).
 bool cluster_allowed(const Problem& p, int cluster) {
     if (cluster == 1) return true;
+    if (p.kind == DG_GEMM_M_GROUPED_RAGGED) return false;                                      // (a pair multiplies its rows with one B)
     if (p.ab_bf16 || p.reduce_batches > 1 || p.a_mn_major || p.b_mn_major) return false;       // (K-major block-scaled operands: what was measured)
     // (measured at M = 4096; smaller GEMMs keep the one-CTA forms their cost model was fitted on)
     return (p.kind == DG_GEMM_DENSE && p.m >= 1024) || p.kind == DG_GEMM_M_GROUPED_CONTIGUOUS;
@@ -276,7 +280,7 @@ Problem swapped(const Problem& p) {
 
 // Whether a dense GEMM may run with its operands swapped (DG_FORCE_SWAP_AB: 1 = whenever this holds, -1 = never)
 bool swap_allowed(const Problem& p) {
-    return p.kind == DG_GEMM_DENSE && !p.a_mn_major && !p.b_mn_major && !p.accumulate &&
+    return p.kind == DG_GEMM_DENSE && p.planes == 1 && !p.a_mn_major && !p.b_mn_major && !p.accumulate &&
            !p.d_fp8 && !p.stochastic && p.reduce_batches <= 1 && p.m <= 128 && p.n >= 128 && env_int("FORCE_SWAP_AB") >= 0 &&
            env_int("FORCE_BLOCK_M") != 256 && env_int("FORCE_BLOCK_K") != 64;
 }
@@ -326,6 +330,7 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
         // 256 rows per CTA: two 128-row MMAs per K-block on one B stage; K not sliced
         if (forced_block_m ? 128 * halves != forced_block_m : (halves == 2 && p.m <= 128)) continue;
         if (halves == 2 && forced_splits > 1) continue;
+        if (p.planes == 2 && (halves == 2 || bk != 128)) continue;      // a stage already holds 256 rows of A: 128 of either plane
         // Stages of 64 elements of K (twice as many, each half the bytes): K-major FP8 operands and unsliced K only.
         // Built and tested, but it measured 0-20 % slower than 128-element stages on every shape tried (the 64-byte
         // rows double the number of L2 requests), so it is used only on request (DG_FORCE_BLOCK_K=64).
@@ -339,7 +344,7 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
         // A dense GEMM with at most 64 rows stages only those rows of A (16, 32 or 64; the box of its tensor map): the
         // bytes saved per stage become more stages, i.e. more of B in flight.  DG_FORCE_A_ROWS=128 keeps whole tiles.
         int a_rows = 0;
-        if (p.kind == DG_GEMM_DENSE && cluster == 1 && halves == 1 && bk >= 128 && !p.a_mn_major && p.reduce_batches <= 1 && p.m <= 64 &&
+        if (p.kind == DG_GEMM_DENSE && cluster == 1 && halves == 1 && bk >= 128 && !p.a_mn_major && p.reduce_batches <= 1 && p.m <= 64 && p.planes == 1 &&
             env_int("FORCE_A_ROWS") != 128)
             a_rows = p.m <= 16 ? 16 : (p.m <= 32 ? 32 : 64);
         int64_t m_blocks;
@@ -347,7 +352,7 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
             m_blocks = static_cast<int64_t>(p.groups) * ceil_div(std::min(std::max(p.expected_m, 1), p.m), tile_m);
         else if (p.kind == DG_GEMM_M_GROUPED_CONTIGUOUS_PSUM && p.expected_m > 0)
             m_blocks = static_cast<int64_t>(p.groups) * ceil_div(std::min(p.expected_m, p.m), tile_m);
-        else if (p.kind == DG_GEMM_M_GROUPED_CONTIGUOUS_PSUM)   // every group may end with a partly filled tile
+        else if (p.kind == DG_GEMM_M_GROUPED_CONTIGUOUS_PSUM || p.kind == DG_GEMM_M_GROUPED_RAGGED)   // every group may end with a partly filled tile
             m_blocks = ceil_div(p.m, tile_m) + p.groups / 2;
         else if (p.kind == DG_GEMM_K_GROUPED_CONTIGUOUS)        // every group has the full tile grid and a share of K
             m_blocks = static_cast<int64_t>(p.groups) * ceil_div(p.m, tile_m);
@@ -384,6 +389,7 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
                 if (splits > 1 && forced_split_cluster != 0 && in_cluster != (forced_split_cluster > 0 ? 1 : 0)) continue;
                 if (in_cluster && (!allow_cluster_split || splits > 8)) continue;
                 if (lim.swapped && splits > 1 && !in_cluster) continue;
+                if (p.planes == 2 && splits > 1 && !in_cluster) continue;      // (no workspace that calls in flight together would share)
                 const int64_t tiles = mn_tiles * splits;
                 // Clusters are placed inside one GPC each, so fewer of them fit than SMs / size suggests
                 const int64_t waves = in_cluster ? ceil_div<int64_t>(mn_tiles, clusters_at_once(splits, num_sms)) : ceil_div<int64_t>(tiles, units);
@@ -398,7 +404,7 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
                 GemmLayout lay{128u * halves, static_cast<uint32_t>(bn), static_cast<uint32_t>(bk), 2,
                                static_cast<uint32_t>(splits > 1 && !in_cluster ? 4 : d_elem), static_cast<uint32_t>(cluster),
                                p.b_mn_major ? 1u : 0u, static_cast<uint32_t>(p.gran_k_a), static_cast<uint32_t>(p.gran_k_b), 0u,
-                               static_cast<uint32_t>(ab_elem), 2u, p.mxf4 ? 1u : 0u, static_cast<uint32_t>(a_rows)};
+                               static_cast<uint32_t>(ab_elem), 2u, p.mxf4 ? 1u : 0u, static_cast<uint32_t>(a_rows), static_cast<uint32_t>(p.planes)};
                 const GemmLayout unfitted = lay;
                 lay = fit_stages(lay, p.kind == DG_GEMM_K_GROUPED_CONTIGUOUS ? 0 : item_kb, max_stages);   // slices may be one K-block
                 if (lay.num_stages <= 2 && env_int("FORCE_STORE_BUFFERS") != 2) {
@@ -429,10 +435,11 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
                 // and its B rows once per 128-row half), and into which no configuration pulled more than ~67 B per cycle
                 // from L2; and the ring of stages, `stages` of which complete per (load latency + MMA time).
                 const double stage_frac = bk / 128.0;
-                const double mma = 2.0 * bn * halves * stage_frac;
-                const double stage_bytes = (128.0 * halves + static_cast<double>(bn) / cluster) * bk;
+                const int a_parts = halves * p.planes;          // 128-row pieces of A per stage, each multiplied with the stage's B
+                const double mma = 2.0 * bn * a_parts * stage_frac;
+                const double stage_bytes = (128.0 * a_parts + static_cast<double>(bn) / cluster) * bk;
                 // (with a CTA pair the peer's tensor core reads this CTA's half of B as well)
-                const double read_bytes = (128.0 * halves + halves * static_cast<double>(bn) / cluster * (cluster == 2 ? 2.0 : 1.0)) * bk;
+                const double read_bytes = (128.0 * a_parts + a_parts * static_cast<double>(bn) / cluster * (cluster == 2 ? 2.0 : 1.0)) * bk;
                 // (55 B per cycle fitted the cluster-reduced candidates: few-tile shapes whose B is read once, from HBM)
                 const double smem_feed = std::max((stage_bytes + read_bytes) / 150.0, stage_bytes / (in_cluster ? 55.0 : 67.0));
                 const double ring = (1500.0 + mma) / model_stages;
@@ -486,7 +493,7 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
     cfg->swap_ab = lim.swapped ? 1 : 0;
     if (cost_out != nullptr) *cost_out = best.cost;
     cfg->num_ctas = best.in_cluster ? static_cast<int>(best.tiles) :
-                    best.cluster * (p.kind == DG_GEMM_M_GROUPED_MASKED || p.kind == DG_GEMM_M_GROUPED_CONTIGUOUS_PSUM
+                    best.cluster * (p.kind == DG_GEMM_M_GROUPED_MASKED || p.kind == DG_GEMM_M_GROUPED_CONTIGUOUS_PSUM || p.kind == DG_GEMM_M_GROUPED_RAGGED
                                         ? units : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(units, best.tiles))));
     cfg->store_buffers = static_cast<int>(best.lay.store_buffers);
     cfg->a_rows = static_cast<int>(best.lay.a_stage_rows());
@@ -553,7 +560,7 @@ GemmLayout layout_of(const Problem& p, const dg_gemm_config_t& cfg) {
                    static_cast<uint32_t>(cfg.cluster_size), p.b_mn_major ? 1u : 0u,
                    static_cast<uint32_t>(p.gran_k_a), static_cast<uint32_t>(p.gran_k_b),
                    item_kb < cfg.num_stages ? 1u : 0u, static_cast<uint32_t>(ab_elem), static_cast<uint32_t>(cfg.store_buffers),
-                   p.mxf4 ? 1u : 0u, cfg.a_rows > 0 && cfg.a_rows < cfg.block_m ? static_cast<uint32_t>(cfg.a_rows) : 0u};
+                   p.mxf4 ? 1u : 0u, cfg.a_rows > 0 && cfg.a_rows < cfg.block_m ? static_cast<uint32_t>(cfg.a_rows) : 0u, static_cast<uint32_t>(p.planes)};
     return lay;
 }
 
@@ -593,6 +600,7 @@ std::string generate_source(const Problem& p, const dg_gemm_config_t& cfg) {
       << "#define DG_MMA_WHOLE_WARP " << env_int("MMA_WHOLE_WARP", 1) << "\n"
       << "#define DG_PRODUCER_WHOLE_WARP " << env_int("PRODUCER_WHOLE_WARP", 1) << "\n"
       << "#define DG_L2_HINT " << env_int("L2_HINT", 0) << "\n"
+      << "#define DG_PLANES " << p.planes << "\n"
       << "#include <dg/gemm_fp8_fp4.cuh>\n";
     return s.str();
 }
@@ -651,8 +659,9 @@ int encode_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uin
 }
 
 int get_kernel(const Problem& p, const dg_gemm_config_t& cfg, dg_kernel_t* kernel) {
-    static const char* names[6] = {"gemm_fp8_fp4_dense", "gemm_fp8_fp4_m_grouped_contiguous", "gemm_fp8_fp4_m_grouped_masked",
-                                   "gemm_fp8_fp4_m_grouped_contiguous_psum", "gemm_fp8_fp4_k_grouped_contiguous", "gemm_fp8_fp4_batched"};
+    static const char* names[7] = {"gemm_fp8_fp4_dense", "gemm_fp8_fp4_m_grouped_contiguous", "gemm_fp8_fp4_m_grouped_masked",
+                                   "gemm_fp8_fp4_m_grouped_contiguous_psum", "gemm_fp8_fp4_k_grouped_contiguous", "gemm_fp8_fp4_batched",
+                                   "gemm_fp8_fp4_m_grouped_ragged"};
     const std::string src = generate_source(cfg.swap_ab ? swapped(p) : p, cfg);
     return dg_jit_compile(names[p.kind], "dg_gemm_fp8_fp4", src.c_str(), "", kernel);
 }
@@ -673,7 +682,7 @@ int get_plan(const Problem& p, Plan* plan) {
                           static_cast<int>(p.d_fp32), static_cast<int>(p.d_fp8), static_cast<int>(p.accumulate), static_cast<int>(p.a_mn_major),
                           static_cast<int>(p.b_mn_major), p.gran_k_a, p.gran_k_b, p.expected_m, static_cast<int>(p.write_padding),
                           static_cast<int>(p.k_psum), static_cast<int>(p.stochastic), p.reduce_batches > 1 ? 1 : 0, dg_get_num_sms(), state().mk_alignment,
-                          static_cast<int>(p.mxf4)};
+                          static_cast<int>(p.mxf4), p.planes};
     // The key is sized from what goes into it: every field of the descriptor and every setting the choice reads
     constexpr size_t kNumFields = sizeof(fields) / sizeof(fields[0]), kNumEnv = sizeof(kEnvNames) / sizeof(kEnvNames[0]);
     using PlanKey = std::array<int, kNumFields + kNumEnv>;
@@ -725,12 +734,15 @@ struct FixedScratch {
     size_t bytes;
 };
 
-int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratch = nullptr) {
+// `plane_rows` > 0: A is split into two planes that many rows apart, with their scale words [K / 128][plane][row] (dg_bf16_fp4.cu)
+int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratch = nullptr, int plane_rows = 0, bool after_producer = false) {
     DG_REQUIRE_ALIVE();
     env_refresh();
     Problem p;
     int rc = validate(kind, a, true, &p);
     if (rc != DG_OK) return rc;
+    DG_REQUIRE((kind == DG_GEMM_M_GROUPED_RAGGED) <= (plane_rows > 0));
+    if (plane_rows > 0) p.planes = 2;
     if (p.m == 0 || p.n == 0) return DG_OK;
     if (p.k == 0) return fail(DG_ERR_INVALID_ARGUMENT, "k == 0 must be handled by the caller (zero or copy D)");
 
@@ -779,7 +791,8 @@ int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratc
         return rc;
     }
     const bool k_grouped = kind == DG_GEMM_K_GROUPED_CONTIGUOUS;
-    const uint64_t a_rows = kind == DG_GEMM_M_GROUPED_MASKED ? static_cast<uint64_t>(p.groups) * p.m : p.m;
+    const uint64_t d_rows_of_m = kind == DG_GEMM_M_GROUPED_MASKED ? static_cast<uint64_t>(p.groups) * p.m : p.m;
+    const uint64_t a_rows = plane_rows > 0 ? static_cast<uint64_t>(2) * plane_rows : d_rows_of_m;
     // k-grouped: one B for all groups (the group selects a slice of K); every group starts a new packed scale row
     const bool one_b = k_grouped || kind == DG_GEMM_BATCHED;        // (batched: the batch is a dimension of its own)
     const uint64_t b_rows = one_b ? p.n : static_cast<uint64_t>(p.groups) * p.n;
@@ -836,8 +849,9 @@ int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratc
         tm_sfa = tm_sfb = tm_a;                  // never used: the BF16 kernel has no scale loads
     } else {
         // (one packed word per row and K-block, two for the 256-element stages of kind::mxf4)
-        if ((rc = encode_2d(&tm_sfa, CU_TENSOR_MAP_DATA_TYPE_INT32, a->sfa, p.m, sfa_rows, a->sfa_pitch * 4, cfg.block_m, lay.sfa_words(),
-                            CU_TENSOR_MAP_SWIZZLE_NONE, nb, bs_sfa)) != DG_OK) return rc;
+        // (split A: two rows per K-block, one for each plane, in one box)
+        if ((rc = encode_2d(&tm_sfa, CU_TENSOR_MAP_DATA_TYPE_INT32, a->sfa, plane_rows > 0 ? plane_rows : p.m, sfa_rows * p.planes, a->sfa_pitch * 4, cfg.block_m,
+                            lay.sfa_words() * p.planes, CU_TENSOR_MAP_SWIZZLE_NONE, nb, bs_sfa)) != DG_OK) return rc;
         if ((rc = encode_2d(&tm_sfb, CU_TENSOR_MAP_DATA_TYPE_INT32, a->sfb, p.n, sfb_rows, a->sfb_pitch * 4, lay.sf_block_n(), lay.sfb_words(),
                             CU_TENSOR_MAP_SWIZZLE_NONE, nb, bs_sfb)) != DG_OK) return rc;
     }
@@ -849,7 +863,7 @@ int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratc
                                        p.d_fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     void* d_base = split ? static_cast<void*>(workspace) : a->d;
     const uint64_t d_rows = split ? static_cast<uint64_t>(cfg.num_splits) * panel_rows :
-                            (k_grouped ? static_cast<uint64_t>(p.groups) * p.m : a_rows);
+                            (k_grouped ? static_cast<uint64_t>(p.groups) * p.m : d_rows_of_m);
     const uint64_t d_pitch_bytes = split ? ld_ws * 4 : a->ldd * (p.d_fp32 ? 4 : (p.d_fp8 ? 1 : 2));
     if (cfg.swap_ab) {
         // The transposed epilogue stages [rows of the caller's D][128 of its columns] blocks (plain row-major, as many rows
@@ -884,6 +898,7 @@ int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratc
     params.sfd = static_cast<uint32_t*>(a->sfd);
     params.sfd_pitch = static_cast<uint32_t>(a->sfd_pitch);
     params.kb_per_batch = static_cast<uint32_t>(k_inner * ab_elem / cfg.block_k);
+    params.plane_rows = static_cast<uint32_t>(plane_rows);
     void* kargs[7] = {&tm_a, &tm_b, &tm_sfa, &tm_sfb, &tm_d, &tm_d_full, &params};
     if (env_int("PROFILE") && fixed_scratch == nullptr) {
         // synchronous, printing path for tuning only (it allocates its counters and waits for the stream, so the entry
@@ -913,7 +928,8 @@ int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratc
                                         static_cast<cudaStream_t>(a->stream));
         return DG_OK;
     }
-    if ((rc = dg_jit_launch(kernel, cfg.num_ctas, 128 + cfg.block_m, launch_cluster, cfg.smem_bytes, state().pdl, a->stream, kargs)) != DG_OK) return rc;
+    // (behind the kernel that splits A always: it lets this one set up early)
+    if ((rc = dg_jit_launch(kernel, cfg.num_ctas, 128 + cfg.block_m, launch_cluster, cfg.smem_bytes, state().pdl || after_producer, a->stream, kargs)) != DG_OK) return rc;
     if (split)
         return launch_splitk_reduce(workspace, a->d, p.m, p.n, ld_ws, panel_rows, a->ldd, cfg.num_splits, alpha, p.d_fp32,
                                     static_cast<cudaStream_t>(a->stream));
@@ -932,6 +948,11 @@ void release_split_workspaces() {
     for (auto& [device, w] : g_workspaces)
         if (w.first != nullptr) cudaFree(w.first);
     g_workspaces.clear();
+}
+
+// Called by dg_bf16_fp4.cu: the GEMM of a split A (args->a, sfa: the planes, plane_rows apart), launched behind the kernel that splits it
+int run_split_a_gemm(const dg_gemm_args_t* args, bool ragged, int plane_rows) {
+    return run_gemm(ragged ? DG_GEMM_M_GROUPED_RAGGED : DG_GEMM_DENSE, args, nullptr, plane_rows, true);
 }
 
 // Called by the no-allocation entry point in dg_splitk.cu, which owns the fixed buffer
@@ -1003,6 +1024,12 @@ int dg_enumerate_tiles(int kind, int block_n, int raster_group, int shape_m, int
             TileScheduler<kMGroupedPsum> sched(128, bn, rg, sm, sn, ng, layout_host, c, nc);
             sched.group_alignment = static_cast<uint32_t>(state().mk_alignment);
             while (sched.next(t)) { t.m_block += t.a_row_base / 128; emit(); }
+            break;
+        }
+        case DG_GEMM_M_GROUPED_RAGGED: {
+            // m_block is reported as the tile's first row of D
+            TileScheduler<kMGroupedRagged> sched(128, bn, rg, sm, sn, ng, layout_host, c, nc);
+            while (sched.next(t)) { t.m_block = t.d_row_base + t.m_block * 128; emit(); }
             break;
         }
         case DG_GEMM_K_GROUPED_CONTIGUOUS: {

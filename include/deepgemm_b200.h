@@ -48,7 +48,8 @@ typedef enum dg_gemm_kind {
     DG_GEMM_M_GROUPED_MASKED = 2,
     DG_GEMM_M_GROUPED_CONTIGUOUS_PSUM = 3,    /* the contiguous layout with use_psum_layout (for dg_get_gemm_config / dg_gemm_precompile) */
     DG_GEMM_K_GROUPED_CONTIGUOUS = 4,
-    DG_GEMM_BATCHED = 5
+    DG_GEMM_BATCHED = 5,
+    DG_GEMM_M_GROUPED_RAGGED = 6              /* groups of any size, no padding: the many-row form of dg_m_grouped_bf16_fp4_gemm_ragged (scheduler model only) */
 } dg_gemm_kind_t;
 
 DG_API const char* dg_last_error(void);
@@ -283,7 +284,7 @@ DG_API int dg_get_gemm_config(int kind, const dg_gemm_args_t* args, dg_gemm_conf
 
 /* Host model of the device tile scheduler (scheduler/gemm.cuh:108-263 in the reference): lists the
  * tiles CTA `cta` of `num_ctas` visits, four uint32 per tile {m_block, n_block, group, valid_rows}
- * (prefix-sum layout: m_block counts from row 0 of A; k-grouped: the fourth word is the slice's K-block count).
+ * (prefix-sum layout: m_block counts from row 0 of A; ragged: m_block is the tile's first row of D; k-grouped: the fourth word is the slice's K-block count).
  * `layout` is a HOST pointer here.  Returns the number of tiles (may exceed max_tiles; only
  * max_tiles are written) or a negative dg_status_t. */
 DG_API int dg_enumerate_tiles(int kind, int block_n, int raster_group, int shape_m, int shape_n, int num_groups,
