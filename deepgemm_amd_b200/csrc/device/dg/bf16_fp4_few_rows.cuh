@@ -11,16 +11,18 @@
 // whose FP32 accumulators are added at the end.  (Unpacking W to FP16 for the register-operand MMA instead costs
 // some 28 instructions per 512 weights, which held a kernel built that way to 3.3 TB/s of W; here no instruction is spent on W.)
 //
-// Work.  W is the 128-row operand: a CTA takes 128 columns of D, up to kTokens rows of A (2 kTokens tile columns) and a share of K.
+// Work.  W is the 128-row operand: an item is 128 columns of D times up to kTokens rows of A (2 kTokens tile columns).  CTAs stay and take
+// items in turn; the accumulators are double, so an item's epilogue runs under the next one's loads and products.
 //   warp 0      TMA producer: per 128 elements of K 128 rows of W (8 KB, unpacked to a byte each on the way), their scale words, and A
 //   warp 1      MMA issuer
-//   warp 2      allocates tensor memory, rearranges the scale words of W for tcgen05.cp
-//   warps 4-7   split the stage's rows of A into its tile columns and their scales; then the epilogue
-// From nine rows on splitting them again in every CTA costs more than the weights (a block of 32 rows took 0.6 us), so a kernel of its own
-// does it once and this one loads the two planes; it asks for the first stages of W before that kernel is done.
-// Where the columns of D alone do not occupy the GPU, the CTAs of a cluster (up to 8) share K and send their partial sums to
-// one another through distributed shared memory, every CTA adding up its own rows of D in rank order.  Two CTAs share an SM
-// (up to 32 rows): one's start and end hide behind the other's stream, and the two MMA loops, each bound by its own latency, add up.
+//   warp 2      allocates tensor memory, rearranges scale words for tcgen05.cp
+//   warps 4-7   epilogue
+//   warps 8-11  split the stage's rows of A into its tile columns and their scales (up to eight rows).  From nine rows on splitting them
+// again in every CTA costs more than the weights (a block of 32 rows took 0.6 us), so a kernel of its own does it once and this one loads the
+// two planes; it asks for the first stages of W before that kernel is done.
+// Where the items alone do not occupy the GPU, the CTAs of a cluster (up to 8) share an item's K and send their partial sums to one another
+// through distributed shared memory, every CTA adding up its own rows of D in rank order.  One CTA's ring of stages takes ~1.5 us to go
+// round (load, split, multiply), 0.3 us per block of 8 KB; two CTAs share an SM, which together ask for what HBM delivers.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -35,11 +37,12 @@ struct Bf16Fp4Params {
     void* d;                     // [m, n], pitch ldd
     const int* group_ends;       // null: one group of m rows
     int* status;                 // host-visible status word, 0 = ok
-    int m, n, k, gran;
+    int m, n, k;
     int64_t ldd;
     int d_fp32, accumulate;
     float alpha;
     int slots;                   // A split ahead: slots per plane (hi, then lo)
+    int groups;
 };
 
 // Rows [first, end) of group g; ends outside [0, m] or before their predecessor give an empty group rather than a wild access
@@ -96,38 +99,91 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const A
     return __all_sync(0xFFFFFFFFu, ok) != 0;
 }
 
+// One thread of the warp, the same one every time
+__device__ __forceinline__ bool elect_one() {
+    uint32_t elected;
+    asm volatile("{.reg .pred p; elect.sync _|p, 0xFFFFFFFF; selp.b32 %0, 1, 0, p;}" : "=r"(elected));
+    return elected != 0;
+}
+// A value that lane `l` holds, to all lanes.  (A reduction rather than a shuffle: its result is known to be the same in the whole warp, so what
+// is computed from it, the MMA's descriptors above all, stays in uniform registers)
+__device__ __forceinline__ int from_lane(int v, int l) { return __reduce_add_sync(0xFFFFFFFFu, static_cast<int>(lane_id()) == l ? v : 0); }
+
+// The items in their order: groups, in a group its blocks of 128 columns, for each of them the passes of kTokens rows.  Lane l of a warp
+// holds group `window + l`, so finding an item takes a ballot, and 32 groups are passed over with one load.
+struct Items {
+    int groups, tiles, tokens, window = -32, before = 0;      // items of the groups ahead of the window
+    int my_first = 0, my_rows = 0, my_end = 0;                // this lane's group: its rows, the items up to and with it
+    int group, first, rows, row, n0;                          // the item: its group, that one's rows, first row of the pass, first column
+
+    __device__ Items(const Bf16Fp4Params& p, int groups_, int tokens_) : groups(groups_), tiles((p.n + 127) / 128), tokens(tokens_) {}
+
+    // The warp together; items in growing order
+    __device__ __forceinline__ bool find(const Bf16Fp4Params& p, int item) {
+        int end = window < 0 ? 0 : from_lane(my_end, 31);
+        while (item >= end) {
+            if (window + 32 >= groups) return false;
+            window += 32;
+            before = end;
+            const int g = window + static_cast<int>(lane_id());
+            int last = 0;
+            my_first = 0;
+            if (g < groups) group_rows(p, g, my_first, last);
+            my_rows = max(last - my_first, 0);
+            my_end = tiles * ((my_rows + tokens - 1) / tokens);
+            #pragma unroll
+            for (int off = 1; off < 32; off *= 2) {
+                const int v = __shfl_up_sync(0xFFFFFFFFu, my_end, off);
+                if (static_cast<int>(lane_id()) >= off) my_end += v;
+            }
+            my_end += before;
+            end = from_lane(my_end, 31);
+        }
+        const int l = __ffs(__ballot_sync(0xFFFFFFFFu, item < my_end)) - 1;
+        group = window + l;
+        first = from_lane(my_first, l);
+        rows = from_lane(my_rows, l);
+        const int passes = (rows + tokens - 1) / tokens, local = item - (from_lane(my_end, l) - tiles * passes);
+        row = first + local % passes * tokens;
+        n0 = local / passes * 128;
+        return true;
+    }
+    __device__ __forceinline__ int rows_here() const { return min(tokens, first + rows - row); }
+};
+
 // kSplit: the kernel splits A itself (a token or a few); otherwise A comes as the two planes of a kernel before this one
 template <int kTokens, bool kSplit> struct Shape {
     static constexpr int kCols = 2 * kTokens;                                // columns of the tile
-    static constexpr int kCtasPerSm = kTokens <= 32 ? 2 : 1;
-    static constexpr int kStages = kTokens == 8 ? 5 : (kTokens == 16 ? 4 : (kTokens == 32 ? 3 : 5));
-    // The splitting warps form teams that take turns at the K-blocks: a block's chain of wait, shuffles, conversions, stores and fence
-    // is long, so as many blocks as possible are at it at once.  Every lane splits four pieces of eight elements of a block
-    static constexpr int kTeam = kTokens / 8, kTeams = 4 / kTeam, kPieces = 4;
-    static constexpr int kThreads = 256;
-    static_assert(!kSplit || (kTeams >= 1 && kTeams <= kStages), "a team that is done with its last block knows that the stage of its next one is at most one block behind");
+    static constexpr int kStages = kTokens == 8 ? 5 : (kTokens == 16 ? 4 : 3), kCtasPerSm = 2;
+    static constexpr int kThreads = kSplit ? 384 : 256;
+    // The splitting warps take turns at the K-blocks: a block's chain of wait, shuffles, conversions, stores and fence is long, so as many
+    // blocks as possible are at it at once.  Every lane splits four pieces of eight elements of a block
+    static constexpr int kSplitWarps = 4, kPieces = 4;
+    static_assert(!kSplit || (kTokens == 8 && kSplitWarps <= kStages), "a warp that is done with its last block knows that the stage of its next one is at most one block behind");
     static constexpr int kOffB = kStages * 16384, kOffA = kOffB + kStages * kCols * 128, kOffSfa = kOffA + (kSplit ? kStages * kTokens * 256 : 0), kOffSfb = kOffSfa + kStages * 512;
-    static constexpr int kOffBar = kOffSfb + kStages * 512, kOffMisc = kOffBar + (4 * kStages + 2) * 8, kOffRecv = (kOffMisc + 8 + 15) / 16 * 16;
-    static constexpr int kTmemCols = kCols + 8 <= 32 ? 32 : (kCols + 8 <= 64 ? 64 : (kCols + 8 <= 128 ? 128 : 256));
+    static constexpr int kOffBar = kOffSfb + kStages * 512, kOffMisc = kOffBar + (4 * kStages + 4) * 8, kOffRecv = (kOffMisc + 8 + 15) / 16 * 16;
+    static constexpr int kTmemCols = 2 * kCols + 8 <= 64 ? 64 : (2 * kCols + 8 <= 128 ? 128 : 256);
     // What a CTA receives: every slice's partial sums of the rows of D it owns
     __host__ __device__ static constexpr int recv_rows(int slices) { return (kTokens + slices - 1) / slices; }
     __host__ __device__ static constexpr int smem_bytes(int slices) { return kOffRecv + (slices > 1 ? slices * recv_rows(slices) * 512 : 0); }
 };
 
-template <int kTokens, bool kSplit>
-__global__ void __launch_bounds__(256, Shape<kTokens, kSplit>::kCtasPerSm)
+// kGran: elements of K per scale of W
+template <int kTokens, bool kSplit, int kGran>
+__global__ void __launch_bounds__(Shape<kTokens, kSplit>::kThreads, Shape<kTokens, kSplit>::kCtasPerSm)
 bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_sf, const __grid_constant__ CUtensorMap tm_a,
                          const __grid_constant__ CUtensorMap tm_sfa, const Bf16Fp4Params p) {
     using S = Shape<kTokens, kSplit>;
     constexpr uint32_t kStages = S::kStages, kCols = S::kCols;
     extern __shared__ __align__(1024) uint8_t smem[];
-    const uint32_t warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x / 32, 0), lane = lane_id();
+    const uint32_t warp = __reduce_max_sync(0xFFFFFFFFu, threadIdx.x / 32), lane = lane_id();
     const uint32_t base = smem_u32(smem);
     auto full_bar = [&](uint32_t s) { return base + S::kOffBar + s * 8; };
     auto sf_bar = [&](uint32_t s) { return base + S::kOffBar + (kStages + s) * 8; };
     auto empty_bar = [&](uint32_t s) { return base + S::kOffBar + (2 * kStages + s) * 8; };
     auto a_bar = [&](uint32_t s) { return base + S::kOffBar + (3 * kStages + s) * 8; };
-    const uint32_t done_bar = base + S::kOffBar + 4 * kStages * 8, free_bar = done_bar + 8;
+    auto done_bar = [&](uint32_t a) { return base + S::kOffBar + (4 * kStages + a) * 8; };
+    auto free_bar = [&](uint32_t a) { return base + S::kOffBar + (4 * kStages + 2 + a) * 8; };
     volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + S::kOffMisc);
     volatile uint32_t* const abort_flag = tmem_slot + 1;
     const AbortCtx ctx{abort_flag, p.status};
@@ -135,23 +191,23 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(slices));
     const uint32_t rank = cluster_ctarank();
 
-    if (threadIdx.x == 0) {
+    if (warp == 0 && lane == 0) {
         *abort_flag = 0;
-        prefetch_tensormap(&tm_w);
-        prefetch_tensormap(&tm_sf);
-        prefetch_tensormap(&tm_a);
-        if (!kSplit) prefetch_tensormap(&tm_sfa);
-    }
-    if (warp == 1 && lane == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
-            mbar_init(full_bar(s), 2 + (kSplit ? S::kTeam : 0));      // the producer, the rearranging warp, a team of splitting warps
+            mbar_init(full_bar(s), 2 + (kSplit ? 1 : 0));      // the producer, the rearranging warp, a splitting warp
             mbar_init(sf_bar(s), 1);
             mbar_init(empty_bar(s), 1);          // tcgen05.commit
             mbar_init(a_bar(s), 1);
         }
-        mbar_init(done_bar, 1);                  // tcgen05.commit: a pass's accumulators are complete
-        mbar_init(free_bar, 4);                  // the epilogue warps have read them
+        for (uint32_t a = 0; a < 2; ++a) {
+            mbar_init(done_bar(a), 1);           // tcgen05.commit: an item's accumulators are complete
+            mbar_init(free_bar(a), 4);           // the epilogue warps have read them
+        }
         fence_mbar_init();
+        prefetch_tensormap(&tm_w);
+        prefetch_tensormap(&tm_sf);
+        prefetch_tensormap(&tm_a);
+        if (!kSplit) prefetch_tensormap(&tm_sfa);
     }
     __syncwarp();
     if (warp == 2) {
@@ -161,17 +217,15 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem = *tmem_slot, tmem_sfa = tmem + kCols, tmem_sfb = tmem_sfa + 4;
+    const uint32_t tmem = __reduce_max_sync(0xFFFFFFFFu, *tmem_slot), tmem_sfa = tmem + 2 * kCols, tmem_sfb = tmem_sfa + 4;
     // With A split ahead, what the kernel before this one wrote is A alone: the producer asks for W before it waits for that kernel (it was
     // itself launched behind everything that came before)
     if (kSplit || warp != 0) griddep_wait();
     griddep_launch_dependents();
 
-    const int group = blockIdx.z, n0 = blockIdx.x / slices * 128;
-    int first, end;
-    group_rows(p, group, first, end);
     const int num_blocks = p.k / 128, per_slice = (num_blocks + slices - 1) / slices;
     const int kb0 = min(static_cast<int>(rank) * per_slice, num_blocks), kb1 = min(kb0 + per_slice, num_blocks);
+    const bool some = kb1 > kb0;                 // (a slice beyond the end of K has nothing to add)
     uint32_t stage = 0, phase = 0;
     auto advance = [&]() {
         stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -179,26 +233,28 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     };
     bool ok = true;
 
-    // Every role walks the same passes (kTokens rows of A each) and K-blocks
-    uint32_t pass = 0, steps = 0;                // (steps: K-blocks of the passes before, for the splitting warps)
-    for (int r0 = first + blockIdx.y * kTokens; r0 < end; r0 += gridDim.y * kTokens, ++pass) {
-        // first half of a split barrier: this CTA runs, and what it received in the pass before has been read
-        __syncwarp();
+    // Every warp walks the same items and K-blocks
+    Items at(p, p.groups, kTokens);
+    const int step = gridDim.x / slices;
+    uint32_t count = 0, steps = 0;               // items so far: accumulator count % 2; their K-blocks (splitting warps)
+    for (int item = blockIdx.x / slices; at.find(p, item); item += step, ++count) {
+        const uint32_t accum = count & 1, accum_phase = count >> 1 & 1;
+        // first half of a split barrier: this CTA runs, and what it received for the item before has been read
         if (slices > 1) cluster_arrive_relaxed();
         if (warp == 0) {
-            const int sf_row = group * ((p.k + 4 * p.gran - 1) / (4 * p.gran));
+            const int sf_row = at.group * ((p.k + 4 * kGran - 1) / (4 * kGran));
             auto load_w = [&](int kb) {
                 mbar_arrive_expect_tx(sf_bar(stage), 512 + (kSplit ? 0 : kCols * 4));
-                tma_load_2d(base + S::kOffSfa + stage * 512, &tm_sf, sf_bar(stage), n0, sf_row + (p.gran == 32 ? kb : kb / 4));
+                tma_load_2d(base + S::kOffSfa + stage * 512, &tm_sf, sf_bar(stage), at.n0, sf_row + (kGran == 32 ? kb : kb / 4));
                 mbar_arrive_expect_tx(full_bar(stage), 128 * 64 + (kSplit ? 0 : kCols * 128));
-                tma_load_2d(base + stage * 16384, &tm_w, full_bar(stage), kb * 128, group * p.n + n0);
+                tma_load_2d(base + stage * 16384, &tm_w, full_bar(stage), kb * 128, at.group * p.n + at.n0);
             };
             auto load_a = [&](int kb) {
                 if constexpr (kSplit) {
                     mbar_arrive_expect_tx(a_bar(stage), kTokens * 256);
-                    tma_load_2d(base + S::kOffA + stage * kTokens * 256, &tm_a, a_bar(stage), kb * 128, r0);
+                    tma_load_2d(base + S::kOffA + stage * kTokens * 256, &tm_a, a_bar(stage), kb * 128, at.row);
                 } else {
-                    const int slot = (p.group_ends != nullptr ? first_slot(first, group) : 0) + r0 - first;
+                    const int slot = (p.group_ends != nullptr ? first_slot(at.first, at.group) : 0) + at.row - at.first;
                     tma_load_2d(base + S::kOffSfb + stage * 512, &tm_sfa, sf_bar(stage), slot, 2 * kb);      // hi's words, then lo's
                     #pragma unroll
                     for (int plane = 0; plane < 2; ++plane)
@@ -206,45 +262,47 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                 }
             };
             int kb = kb0;
-            if (!kSplit && pass == 0) {
+            if (!kSplit && count == 0) {
                 // every stage is free: W for all of them, then the kernel before this one, then A
                 const int ahead = min(kb0 + static_cast<int>(kStages), kb1);
                 for (; kb < ahead; ++kb, advance())
-                    if (lane == 0) load_w(kb);
+                    if (elect_one()) load_w(kb);
                 __syncwarp();
                 griddep_wait();
                 stage = 0;
                 for (int b = kb0; b < ahead; ++b, ++stage)
-                    if (lane == 0) load_a(b);
+                    if (elect_one()) load_a(b);
                 stage = (ahead - kb0) % kStages;
                 __syncwarp();
             }
             for (; ok && kb < kb1; ++kb, advance()) {
                 if (!(ok = warp_wait(empty_bar(stage), phase ^ 1, ctx, 1))) break;
-                if (lane == 0) {
-                    load_w(kb);
+                if (elect_one()) {
                     load_a(kb);
+                    load_w(kb);
                 }
                 __syncwarp();
             }
         } else if (warp == 1) {
             constexpr uint32_t idesc = make_instr_desc_block_scaled(kFmtE2M1, kFmtE4M3, 0, 0, 128, kCols);
-            ok = ok && warp_wait(free_bar, (pass & 1) ^ 1, ctx, 2);
+            if (some) ok = ok && warp_wait(free_bar(accum), accum_phase ^ 1, ctx, 2);
             tc_fence_after_sync();
             for (int kb = kb0; ok && kb < kb1; ++kb, advance()) {
                 if (!(ok = warp_wait(full_bar(stage), phase, ctx, 2))) break;
                 tc_fence_after_sync();
-                if (lane == 0) {
-                    tc_cp_32x128b_warpx4<1>(tmem_sfa, make_smem_desc(base + S::kOffSfa + stage * 512, 0, 128, kSwizzleNone));
-                    tc_cp_32x128b_warpx4<1>(tmem_sfb, make_smem_desc(base + S::kOffSfb + stage * 512, 0, 128, kSwizzleNone));
-                    const uint64_t a_desc = make_smem_desc(base + stage * 16384, 0, 1024, kSwizzle128B);
-                    const uint64_t b_desc = make_smem_desc(base + S::kOffB + stage * kCols * 128, 0, 1024, kSwizzle128B);
+                const uint64_t a_desc = make_smem_desc(base + stage * 16384, 0, 1024, kSwizzle128B);
+                const uint64_t b_desc = make_smem_desc(base + S::kOffB + stage * kCols * 128, 0, 1024, kSwizzle128B);
+                const uint64_t sfa_desc = make_smem_desc(base + S::kOffSfa + stage * 512, 0, 128, kSwizzleNone);
+                const uint64_t sfb_desc = make_smem_desc(base + S::kOffSfb + stage * 512, 0, 128, kSwizzleNone);
+                if (elect_one()) {
+                    tc_cp_32x128b_warpx4<1>(tmem_sfa, sfa_desc);
+                    tc_cp_32x128b_warpx4<1>(tmem_sfb, sfb_desc);
                     #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j)
-                        tc_mma_mxf8f6f4<1>(tmem, a_desc + j * 2, b_desc + j * 2, instr_desc_with_sf_ids(idesc, p.gran == 32 ? j : kb % 4, j), tmem_sfa, tmem_sfb,
-                                           kb != kb0 || j != 0);
+                        tc_mma_mxf8f6f4<1>(tmem + accum * kCols, a_desc + j * 2, b_desc + j * 2, instr_desc_with_sf_ids(idesc, kGran == 32 ? j : kb % 4, j),
+                                           tmem_sfa, tmem_sfb, kb != kb0 || j != 0);
                     tc_commit(empty_bar(stage));
-                    if (kb + 1 == kb1) tc_commit(done_bar);
+                    if (kb + 1 == kb1) tc_commit(done_bar(accum));
                 }
                 __syncwarp();
             }
@@ -252,32 +310,35 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
             // tcgen05.cp puts row r of 32 x 16 bytes into lane r: the word of tile row 32 c + r has to sit at word 4 r + c
             for (int kb = kb0; ok && kb < kb1; ++kb, advance()) {
                 if (!(ok = warp_wait(sf_bar(stage), phase, ctx, 3))) break;
-                const uint32_t words = base + S::kOffSfa + stage * 512;
-                uint32_t v[4];
+                const uint32_t words = base + S::kOffSfa + stage * 512, own = base + S::kOffSfb + stage * 512;
+                uint32_t v[4], w[4];
                 #pragma unroll
                 for (uint32_t c = 0; c < 4; ++c) v[c] = ld_shared_u32(words + (c * 32 + lane) * 4);
+                if constexpr (!kSplit) {                                     // the same for the scale words of A (the splitting warps write theirs in place)
+                    #pragma unroll
+                    for (uint32_t c = 0; c < 4; ++c) w[c] = c * 32 < kCols ? ld_shared_u32(own + (c * 32 + lane) * 4) : 0u;
+                }
                 __syncwarp();
                 st_shared_v4(words + lane * 16, v[0], v[1], v[2], v[3]);
-                if constexpr (!kSplit) {                                     // the same for the scale words of A (the splitting warps write theirs in place)
-                    const uint32_t own = base + S::kOffSfb + stage * 512;
-                    #pragma unroll
-                    for (uint32_t c = 0; c < 4; ++c) v[c] = c * 32 < kCols ? ld_shared_u32(own + (c * 32 + lane) * 4) : 0u;
-                    __syncwarp();
-                    st_shared_v4(own + lane * 16, v[0], v[1], v[2], v[3]);
-                }
+                if constexpr (!kSplit) st_shared_v4(own + lane * 16, w[0], w[1], w[2], w[3]);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full_bar(stage));
+                __syncwarp();
             }
-        } else if (kSplit && warp >= 4) {
-            const int rows = min(kTokens, end - r0), blocks = kb1 - kb0;
-            const int team = (warp - 4) / S::kTeam, member = (warp - 4) % S::kTeam;
-            // Piece i of this lane: elements 8 (lane % 16) .. of the K-block, of row 2 (i kTeam + member) + lane / 16
-            const int row0 = member * 2 + lane / 16, chunk = lane % 16;
-            for (int b = team; ok && b < blocks; b += S::kTeams) {
-                const uint32_t at_stage = (steps + b) % kStages, at_phase = (steps + b) / kStages & 1;
+        } else if (warp >= 8) {
+            const int rows = at.rows_here(), blocks = kb1 - kb0, turn = warp - 8;
+            // Piece i of this lane: elements 8 (lane % 16) .. of the K-block, of row 2 i + lane / 16.  (stage, phase: those of the item's first block)
+            const int row0 = lane / 16, chunk = lane % 16;
+            uint32_t b_stage = stage, b_phase = phase;
+            for (int b = 0; ok && b < blocks; ++b) {
+                const uint32_t at_stage = b_stage, at_phase = b_phase;
+                b_stage = b_stage + 1 == kStages ? 0 : b_stage + 1;
+                b_phase ^= b_stage == 0;
+                // (counted over all items: a warp is then never more than kSplitWarps blocks away from its last one)
+                if ((steps + b) % S::kSplitWarps != static_cast<uint32_t>(turn)) continue;
                 // First that the stage's block before this one has been multiplied, then that this one's A has landed.  Copies land in any
-                // order, and a team that only asked for the latter could ask while the copy of the block before is still
+                // order, and a warp that only asked for the latter could ask while the copy of the block before is still
                 // under way: a barrier two phases behind answers like one that is done.
                 if (!(ok = warp_wait(empty_bar(at_stage), at_phase ^ 1, ctx, kRoleSplit))) break;
                 if (!(ok = warp_wait(a_bar(at_stage), at_phase, ctx, kRoleSplit))) break;
@@ -286,97 +347,102 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                 uint8_t* const sf = smem + S::kOffSfb + at_stage * 512;
                 #pragma unroll
                 for (int i = 0; i < S::kPieces; ++i) {
-                    if (2 * (S::kTeam * i + member) < rows) {                // (a row beyond the last one beside it: its columns are not stored)
-                        const int row = row0 + 2 * S::kTeam * i, col = kTokens + row;
+                    if (2 * i < rows) {                                      // (a row beyond the last one beside it: its columns are not stored)
+                        const int row = row0 + 2 * i, col = kTokens + row;
                         uint2 hi, lo;
                         const uint32_t code = split_bf16(*reinterpret_cast<const uint4*>(a + row * 256), hi, lo);
-                        const int at = (((chunk / 2) ^ (row & 7)) << 4) + chunk % 2 * 8;
-                        *reinterpret_cast<uint2*>(tile + row * 128 + at) = hi;
-                        *reinterpret_cast<uint2*>(tile + col * 128 + at) = lo;
+                        const int to = (((chunk / 2) ^ (row & 7)) << 4) + chunk % 2 * 8;
+                        *reinterpret_cast<uint2*>(tile + row * 128 + to) = hi;
+                        *reinterpret_cast<uint2*>(tile + col * 128 + to) = lo;
                         if (chunk % 4 == 0) {
-                            sf[row % 32 * 16 + row / 32 * 4 + chunk / 4] = static_cast<uint8_t>(code);
-                            sf[col % 32 * 16 + col / 32 * 4 + chunk / 4] = static_cast<uint8_t>(code == 255 ? 255 : code - 4);
+                            sf[row * 16 + chunk / 4] = static_cast<uint8_t>(code);
+                            sf[col * 16 + chunk / 4] = static_cast<uint8_t>(code == 255 ? 255 : code - 4);
                         }
                     }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full_bar(at_stage));
+                __syncwarp();
             }
+            stage = b_stage;
+            phase = b_phase;
             steps += blocks;
-        }
-        if (warp >= 4) {
-            const int rows = min(kTokens, end - r0);
-            // Epilogue: this thread's column of D, rows r0 .. r0 + rows
+        } else if (warp >= 4) {
+            // Epilogue: this thread's column of D, the pass's rows of it
+            const int rows = at.rows_here(), r0 = at.row;
             const uint32_t quarter = warp % 4, row = quarter * 32 + lane;
-            const int n = n0 + static_cast<int>(row);
+            const int n = at.n0 + static_cast<int>(row);
             auto write = [&](int t, float y) {
                 if (t >= rows || n >= p.n) return;
-                const int64_t at = static_cast<int64_t>(r0 + t) * p.ldd + n;
+                const int64_t to = static_cast<int64_t>(r0 + t) * p.ldd + n;
                 y *= p.alpha;
                 if (p.d_fp32) {
-                    float* const out = static_cast<float*>(p.d) + at;
+                    float* const out = static_cast<float*>(p.d) + to;
                     *out = p.accumulate ? *out + y : y;
                 } else {
-                    __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.d) + at;
+                    __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.d) + to;
                     if (p.accumulate) y += __bfloat162float(*out);
                     *out = __float2bfloat16_rn(y);
                 }
             };
-            const bool some = kb1 > kb0;                                     // (a slice beyond the end of K has nothing to add)
-            if (ok && some) ok = warp_wait(done_bar, pass & 1, ctx, 4);
+            if (ok && some) ok = warp_wait(done_bar(accum), accum_phase, ctx, 4);
             tc_fence_after_sync();
             const uint32_t own_rows = S::recv_rows(slices), recv = base + S::kOffRecv;
-            __syncwarp();
-            if (slices > 1) cluster_wait();                                  // every CTA of the cluster may be written to
-            uint32_t owner = 0, at_owner = 0;                                // row t of D: CTA t mod slices, its (t / slices)-th
+            float y[kTokens];
             #pragma unroll
             for (int t0 = 0; t0 < kTokens; t0 += 16) {
                 uint32_t v[16], w[16];
-                __syncwarp();                                                // (lanes beyond N skip the stores)
                 if (some) {
-                    tmem_ld_32x32b_x16(tmem + ((quarter * 32) << 16) + t0, v);
-                    if constexpr (kTokens >= 16) tmem_ld_32x32b_x16(tmem + ((quarter * 32) << 16) + kTokens + t0, w);
+                    tmem_ld_32x32b_x16(tmem + ((quarter * 32) << 16) + accum * kCols + t0, v);
+                    if constexpr (kTokens >= 16) tmem_ld_32x32b_x16(tmem + ((quarter * 32) << 16) + accum * kCols + kTokens + t0, w);
                     tmem_ld_wait();
                 }
                 #pragma unroll
-                for (int i = 0; i < (kTokens < 16 ? kTokens : 16); ++i) {
-                    const int t = t0 + i;
-                    const float y = !some ? 0.0f : __uint_as_float(v[i]) + __uint_as_float(kTokens >= 16 ? w[i] : v[i + 8]);
-                    if (slices == 1) {
-                        write(t, y);
-                    } else if (t < rows) {
-                        st_shared_cluster_u32(map_to_cta(recv + ((rank * own_rows + at_owner) * 128 + row) * 4, owner), __float_as_uint(y));
+                for (int i = 0; i < (kTokens < 16 ? kTokens : 16); ++i)
+                    y[t0 + i] = !some ? 0.0f : __uint_as_float(v[i]) + __uint_as_float(kTokens >= 16 ? w[i] : v[i + 8]);
+            }
+            if (some) {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(free_bar(accum));
+            }
+            __syncwarp();
+            if (slices == 1) {
+                #pragma unroll
+                for (int t = 0; t < kTokens; ++t) write(t, y[t]);
+            } else {
+                cluster_wait();                                              // every CTA of the cluster may be written to
+                uint32_t owner = 0, at_owner = 0;                            // row t of D: CTA t mod slices, its (t / slices)-th
+                #pragma unroll
+                for (int t = 0; t < kTokens; ++t) {
+                    if (t < rows) {
+                        st_shared_cluster_u32(map_to_cta(recv + ((rank * own_rows + at_owner) * 128 + row) * 4, owner), __float_as_uint(y[t]));
                         if (++owner == slices) {
                             owner = 0;
                             ++at_owner;
                         }
                     }
                 }
-            }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(free_bar);
-            __syncwarp();                                                    // (the cluster barrier wants the warp together)
-            if (slices > 1) {
+                __syncwarp();
                 cluster_arrive();                                            // release: what this CTA sent is visible to its owners
                 cluster_wait();
                 for (uint32_t i = 0; i < own_rows; ++i) {
                     const int t = static_cast<int>(i * slices + rank);
                     if (t >= rows) break;
-                    float part[kMaxCluster], y = 0.0f;                       // (all loads on their way before the first sum)
+                    float part[kMaxCluster], sum = 0.0f;                     // (all loads on their way before the first sum)
                     #pragma unroll
                     for (uint32_t s = 0; s < kMaxCluster; ++s)
                         part[s] = s < slices ? __uint_as_float(ld_shared_u32(recv + ((s * own_rows + i) * 128 + row) * 4)) : 0.0f;
                     #pragma unroll
-                    for (uint32_t s = 0; s < kMaxCluster; ++s) y += part[s];
-                    write(t, y);
+                    for (uint32_t s = 0; s < kMaxCluster; ++s) sum += part[s];
+                    write(t, sum);
                 }
             }
         }
-        if (slices > 1 && warp < 4) {
-            // the role warps only take part in the two barriers of the epilogue
-            __syncwarp();
+        __syncwarp();                            // (what follows wants every warp together: lanes beyond N skipped stores)
+        if (slices > 1 && (warp < 4 || warp >= 8)) {
+            // the other warps only take part in the two barriers of the epilogue
             cluster_wait();
             cluster_arrive();
             cluster_wait();

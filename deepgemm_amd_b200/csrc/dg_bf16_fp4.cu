@@ -18,16 +18,21 @@ int run_split_a_gemm(const dg_gemm_args_t* args, bool ragged, int plane_rows);  
 
 namespace {
 
-// CTAs along K (a cluster) of a launch with `tiles` CTAs of 128 columns.  What a choice costs: the waves it takes (clusters live inside one
-// GPC, so fewer fit than SMs / size), times a CTA's K-blocks at ~0.2 us and ~3 us to start and end, a little more with partners.
-// (Clusters at once: what a 148-SM B200 reported for one CTA per SM; 32 clusters of 8 where 30 fit took twice the time of 6.)
-int choose_slices(int64_t tiles, int ctas_per_sm, int num_blocks) {
-    static const int kFit[few::kMaxCluster + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+// Clusters of S CTAs that run at once with two CTAs on an SM: what 148-SM B200s showed (a cluster lives inside one GPC, and a few SMs belong to
+// none that takes more than two)
+int clusters_at_once(int slices) {
+    static const int kFit[few::kMaxCluster + 1] = {0, 296, 148, 92, 70, 55, 44, 36, 31};
+    return std::max(1, kFit[slices] * dg_get_num_sms() / 148);
+}
+
+// CTAs along K (a cluster) for a launch with `items` blocks of 128 columns: the number with the fewest K-blocks in a row (~0.3 us each, an
+// SM's two CTAs side by side), a little more with partners, which finish an item before they begin the next
+int choose_slices(int64_t items, int num_blocks) {
     int best = 1;
     double best_cost = 0.0;
     for (int s = 1; s <= few::kMaxCluster && (s == 1 || num_blocks / s >= 2); ++s) {
-        const int64_t at_once = std::max<int64_t>(1, static_cast<int64_t>(kFit[s]) * ctas_per_sm * dg_get_num_sms() / 148);
-        const double cost = static_cast<double>(ceil_div(tiles, at_once)) * (0.2 * ceil_div(num_blocks, s) + 3.0 + (s > 1 ? 0.3 : 0.0));
+        const double waves = static_cast<double>(ceil_div<int64_t>(items, clusters_at_once(s)));
+        const double cost = waves * (0.3 * ceil_div(num_blocks, s) + (s > 1 ? 1.5 : 0.0));
         if (s == 1 || cost < best_cost) {
             best = s;
             best_cost = cost;
@@ -124,8 +129,10 @@ int split_rows(const dg_gemm_args_t* g, const int* group_ends, const Planes& pla
 template <int kTokens, bool kSplit>
 int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Planes& planes) {
     using S = few::Shape<kTokens, kSplit>;
-    const int tiles_n = ceil_div(g->n, 128), passes = p.group_ends != nullptr ? 1 : ceil_div(g->m, kTokens);
-    const int slices = choose_slices(static_cast<int64_t>(tiles_n) * passes * g->num_groups, S::kCtasPerSm, g->k / 128);
+    // Items: exact for a dense product; a ragged one has at most one group per row, and a pass more per kTokens rows
+    const int64_t tiles_n = ceil_div(g->n, 128), passes = ceil_div(g->m, kTokens);
+    const int64_t items = tiles_n * (p.group_ends != nullptr ? std::min(g->m, g->num_groups + g->m / kTokens) : passes);
+    const int slices = choose_slices(items, g->k / 128);
     CUtensorMap tm_w, tm_sf, tm_a, tm_sfa;
     int rc;
     const uint64_t words = ceil_div(g->k, 4 * g->gran_k_b);
@@ -143,11 +150,11 @@ int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Plane
                                        static_cast<uint64_t>(planes.slots) * 4, kTokens, 2, CU_TENSOR_MAP_SWIZZLE_NONE)) != DG_OK) return rc;
         if ((rc = split_rows(g, p.group_ends, planes)) != DG_OK) return rc;
     }
-    const auto kernel = few::bf16_fp4_few_rows_kernel<kTokens, kSplit>;
+    const auto kernel = g->gran_k_b == 32 ? few::bf16_fp4_few_rows_kernel<kTokens, kSplit, 32> : few::bf16_fp4_few_rows_kernel<kTokens, kSplit, 128>;
     const int smem = S::smem_bytes(slices);
     DG_CUDA_RT(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(tiles_n * slices, passes, g->num_groups);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items, clusters_at_once(slices))) * slices);
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(g->stream);
@@ -218,8 +225,8 @@ int run(const dg_gemm_args_t* g, bool ragged, void* workspace, int64_t given_byt
     if (rc != DG_OK) return rc;
     const int slots = num_slots(g->m, g->num_groups, ragged), rows = typical_rows(g, ragged);
     const Planes planes{static_cast<uint8_t*>(workspace), reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + static_cast<size_t>(2) * slots * g->k), slots};
-    const Bf16Fp4Params p{g->d, ragged ? g->grouped_layout : nullptr, state().status_device, g->m, g->n, g->k, g->gran_k_b, g->ldd, g->d_dtype == DG_FP32,
-                          g->accumulate != 0, g->has_alpha ? g->alpha : 1.0f, slots};
+    const Bf16Fp4Params p{g->d, ragged ? g->grouped_layout : nullptr, state().status_device, g->m, g->n, g->k, g->ldd, g->d_dtype == DG_FP32,
+                          g->accumulate != 0, g->has_alpha ? g->alpha : 1.0f, slots, g->num_groups};
     if (splits_inside(g, ragged)) return launch_few_rows<8, true>(g, p, planes);
     if (rows <= 16) return launch_few_rows<16, false>(g, p, planes);
     // (the GEMM kernel stores whole 16-byte pieces of a row of D: where N ends inside one, what follows the row would not stay)
