@@ -116,10 +116,19 @@ struct Items {
     int my_first = 0, my_rows = 0, my_end = 0;                // this lane's group: its rows, the items up to and with it
     int group, first, rows, row, n0;                          // the item: its group, that one's rows, first row of the pass, first column
 
-    __device__ Items(const Bf16Fp4Params& p, int groups_, int tokens_) : groups(groups_), tiles((p.n + 127) / 128), tokens(tokens_) {}
+    __device__ Items(const Bf16Fp4Params& p, int groups_, int tokens_) : groups(groups_), tiles((p.n + 127) / 128), tokens(tokens_) {
+        group = first = row = 0;
+        rows = p.m;
+    }
 
     // The warp together; items in growing order
     __device__ __forceinline__ bool find(const Bf16Fp4Params& p, int item) {
+        if (p.group_ends == nullptr) {                        // one group: no search
+            const int passes = (rows + tokens - 1) / tokens, tile = passes == 1 ? item : item / passes;
+            row = (item - tile * passes) * tokens;
+            n0 = tile * 128;
+            return tile < tiles;
+        }
         int end = window < 0 ? 0 : from_lane(my_end, 31);
         while (item >= end) {
             if (window + 32 >= groups) return false;
@@ -154,15 +163,15 @@ struct Items {
 // kSplit: the kernel splits A itself (a token or a few); otherwise A comes as the two planes of a kernel before this one
 template <int kTokens, bool kSplit> struct Shape {
     static constexpr int kCols = 2 * kTokens;                                // columns of the tile
-    static constexpr int kStages = kTokens == 8 ? 5 : (kTokens == 16 ? 4 : 3), kCtasPerSm = 2;
-    static constexpr int kThreads = kSplit ? 384 : 256;
-    // The splitting warps take turns at the K-blocks: a block's chain of wait, shuffles, conversions, stores and fence is long, so as many
-    // blocks as possible are at it at once.  Every lane splits four pieces of eight elements of a block
-    static constexpr int kSplitWarps = 4, kPieces = 4;
-    static_assert(!kSplit || (kTokens == 8 && kSplitWarps <= kStages), "a warp that is done with its last block knows that the stage of its next one is at most one block behind");
+    static constexpr int kStages = kTokens == 8 ? 5 : (kTokens == 16 ? 4 : (kTokens == 32 ? 3 : 5)), kCtasPerSm = kTokens <= 32 ? 2 : 1;
+    // Teams of splitting warps take turns at the K-blocks: a block's chain of wait, shuffles, conversions, stores and fence is long, so as
+    // many blocks as possible are at it at once.  Every lane splits four pieces of eight elements of a block
+    static constexpr int kTeams = 4, kTeam = kTokens / 8, kPieces = 4, kSplitWarps = kTeams * kTeam;
+    static constexpr int kThreads = kSplit ? 256 + 32 * kSplitWarps : 256;
+    static_assert(!kSplit || (kTokens <= 16 && kTeams <= kStages), "a team that is done with its last block knows that the stage of its next one is at most one block behind");
     static constexpr int kOffB = kStages * 16384, kOffA = kOffB + kStages * kCols * 128, kOffSfa = kOffA + (kSplit ? kStages * kTokens * 256 : 0), kOffSfb = kOffSfa + kStages * 512;
     static constexpr int kOffBar = kOffSfb + kStages * 512, kOffMisc = kOffBar + (4 * kStages + 4) * 8, kOffRecv = (kOffMisc + 8 + 15) / 16 * 16;
-    static constexpr int kTmemCols = 2 * kCols + 8 <= 64 ? 64 : (2 * kCols + 8 <= 128 ? 128 : 256);
+    static constexpr int kTmemCols = 2 * kCols + 8 <= 64 ? 64 : (2 * kCols + 8 <= 128 ? 128 : (2 * kCols + 8 <= 256 ? 256 : 512));
     // What a CTA receives: every slice's partial sums of the rows of D it owns
     __host__ __device__ static constexpr int recv_rows(int slices) { return (kTokens + slices - 1) / slices; }
     __host__ __device__ static constexpr int smem_bytes(int slices) { return kOffRecv + (slices > 1 ? slices * recv_rows(slices) * 512 : 0); }
@@ -191,88 +200,91 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(slices));
     const uint32_t rank = cluster_ctarank();
 
-    if (warp == 0 && lane == 0) {
-        *abort_flag = 0;
-        for (uint32_t s = 0; s < kStages; ++s) {
-            mbar_init(full_bar(s), 2 + (kSplit ? 1 : 0));      // the producer, the rearranging warp, a splitting warp
-            mbar_init(sf_bar(s), 1);
-            mbar_init(empty_bar(s), 1);          // tcgen05.commit
-            mbar_init(a_bar(s), 1);
-        }
-        for (uint32_t a = 0; a < 2; ++a) {
-            mbar_init(done_bar(a), 1);           // tcgen05.commit: an item's accumulators are complete
-            mbar_init(free_bar(a), 4);           // the epilogue warps have read them
-        }
-        fence_mbar_init();
-        prefetch_tensormap(&tm_w);
-        prefetch_tensormap(&tm_sf);
-        prefetch_tensormap(&tm_a);
-        if (!kSplit) prefetch_tensormap(&tm_sfa);
-    }
-    __syncwarp();
-    if (warp == 2) {
-        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
-        tmem_relinquish<1>();
-    }
-    tc_fence_before_sync();
-    __syncthreads();
-    tc_fence_after_sync();
-    const uint32_t tmem = __reduce_max_sync(0xFFFFFFFFu, *tmem_slot), tmem_sfa = tmem + 2 * kCols, tmem_sfb = tmem_sfa + 4;
-    // With A split ahead, what the kernel before this one wrote is A alone: the producer asks for W before it waits for that kernel (it was
-    // itself launched behind everything that came before)
-    if (kSplit || warp != 0) griddep_wait();
-    griddep_launch_dependents();
-
     const int num_blocks = p.k / 128, per_slice = (num_blocks + slices - 1) / slices;
     const int kb0 = min(static_cast<int>(rank) * per_slice, num_blocks), kb1 = min(kb0 + per_slice, num_blocks);
     const bool some = kb1 > kb0;                 // (a slice beyond the end of K has nothing to add)
+    const int step = gridDim.x / slices, first_item = blockIdx.x / slices;
+    Items at(p, p.groups, kTokens);
     uint32_t stage = 0, phase = 0;
     auto advance = [&]() {
         stage = stage + 1 == kStages ? 0 : stage + 1;
         phase ^= stage == 0;
     };
+    // The copies of K-block kb of the item into the current stage (one thread)
+    auto load_w = [&](int kb) {
+        mbar_arrive_expect_tx(sf_bar(stage), 512 + (kSplit ? 0 : kCols * 4));
+        tma_load_2d(base + S::kOffSfa + stage * 512, &tm_sf, sf_bar(stage), at.n0, at.group * ((p.k + 4 * kGran - 1) / (4 * kGran)) + (kGran == 32 ? kb : kb / 4));
+        mbar_arrive_expect_tx(full_bar(stage), 128 * 64 + (kSplit ? 0 : kCols * 128));
+        tma_load_2d(base + stage * 16384, &tm_w, full_bar(stage), kb * 128, at.group * p.n + at.n0);
+    };
+    auto load_a = [&](int kb) {
+        if constexpr (kSplit) {
+            mbar_arrive_expect_tx(a_bar(stage), kTokens * 256);
+            tma_load_2d(base + S::kOffA + stage * kTokens * 256, &tm_a, a_bar(stage), kb * 128, at.row);
+        } else {
+            const int slot = (p.group_ends != nullptr ? first_slot(at.first, at.group) : 0) + at.row - at.first;
+            tma_load_2d(base + S::kOffSfb + stage * 512, &tm_sfa, sf_bar(stage), slot, 2 * kb);      // hi's words, then lo's
+            #pragma unroll
+            for (int plane = 0; plane < 2; ++plane)
+                tma_load_2d(base + S::kOffB + stage * kCols * 128 + plane * kTokens * 128, &tm_a, full_bar(stage), kb * 128, plane * p.slots + slot);
+        }
+    };
+
+    // The producer asks for the first item's first stages (all of them free) while the others still set up.  With A split ahead, what the
+    // kernel before this one wrote is A alone, so W is asked for before that kernel is waited for (it was itself launched behind everything
+    // that came before); A follows below.
+    int ahead = kb0;                             // K-blocks of the first item asked for here
+    if (warp == 0) {
+        if (lane == 0) {
+            *abort_flag = 0;
+            for (uint32_t s = 0; s < kStages; ++s) {
+                mbar_init(full_bar(s), 2 + (kSplit ? S::kTeam : 0));       // the producer, the rearranging warp, a team of splitting warps
+                mbar_init(sf_bar(s), 1);
+                mbar_init(empty_bar(s), 1);      // tcgen05.commit
+                mbar_init(a_bar(s), 1);
+            }
+            for (uint32_t a = 0; a < 2; ++a) {
+                mbar_init(done_bar(a), 1);       // tcgen05.commit: an item's accumulators are complete
+                mbar_init(free_bar(a), 4);       // the epilogue warps have read them
+            }
+            fence_mbar_init();
+        }
+        __syncwarp();
+        if (kSplit) griddep_wait();
+        if (at.find(p, first_item)) {
+            ahead = min(kb0 + static_cast<int>(kStages), kb1);
+            for (int kb = kb0; kb < ahead; ++kb, ++stage) {
+                if (elect_one()) {
+                    if (kSplit) load_a(kb);
+                    load_w(kb);
+                }
+            }
+            stage = 0;
+        }
+    } else if (warp == 2) {
+        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
+        tmem_relinquish<1>();
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = __reduce_max_sync(0xFFFFFFFFu, *tmem_slot), tmem_sfa = tmem + 2 * kCols, tmem_sfb = tmem_sfa + 4;
+    griddep_wait();
+    griddep_launch_dependents();
     bool ok = true;
 
     // Every warp walks the same items and K-blocks
-    Items at(p, p.groups, kTokens);
-    const int step = gridDim.x / slices;
     uint32_t count = 0, steps = 0;               // items so far: accumulator count % 2; their K-blocks (splitting warps)
-    for (int item = blockIdx.x / slices; at.find(p, item); item += step, ++count) {
+    for (int item = first_item; at.find(p, item); item += step, ++count) {
         const uint32_t accum = count & 1, accum_phase = count >> 1 & 1;
         // first half of a split barrier: this CTA runs, and what it received for the item before has been read
         if (slices > 1) cluster_arrive_relaxed();
         if (warp == 0) {
-            const int sf_row = at.group * ((p.k + 4 * kGran - 1) / (4 * kGran));
-            auto load_w = [&](int kb) {
-                mbar_arrive_expect_tx(sf_bar(stage), 512 + (kSplit ? 0 : kCols * 4));
-                tma_load_2d(base + S::kOffSfa + stage * 512, &tm_sf, sf_bar(stage), at.n0, sf_row + (kGran == 32 ? kb : kb / 4));
-                mbar_arrive_expect_tx(full_bar(stage), 128 * 64 + (kSplit ? 0 : kCols * 128));
-                tma_load_2d(base + stage * 16384, &tm_w, full_bar(stage), kb * 128, at.group * p.n + at.n0);
-            };
-            auto load_a = [&](int kb) {
-                if constexpr (kSplit) {
-                    mbar_arrive_expect_tx(a_bar(stage), kTokens * 256);
-                    tma_load_2d(base + S::kOffA + stage * kTokens * 256, &tm_a, a_bar(stage), kb * 128, at.row);
-                } else {
-                    const int slot = (p.group_ends != nullptr ? first_slot(at.first, at.group) : 0) + at.row - at.first;
-                    tma_load_2d(base + S::kOffSfb + stage * 512, &tm_sfa, sf_bar(stage), slot, 2 * kb);      // hi's words, then lo's
-                    #pragma unroll
-                    for (int plane = 0; plane < 2; ++plane)
-                        tma_load_2d(base + S::kOffB + stage * kCols * 128 + plane * kTokens * 128, &tm_a, full_bar(stage), kb * 128, plane * p.slots + slot);
-                }
-            };
             int kb = kb0;
-            if (!kSplit && count == 0) {
-                // every stage is free: W for all of them, then the kernel before this one, then A
-                const int ahead = min(kb0 + static_cast<int>(kStages), kb1);
+            if (count == 0) {
                 for (; kb < ahead; ++kb, advance())
-                    if (elect_one()) load_w(kb);
-                __syncwarp();
-                griddep_wait();
-                stage = 0;
-                for (int b = kb0; b < ahead; ++b, ++stage)
-                    if (elect_one()) load_a(b);
-                stage = (ahead - kb0) % kStages;
+                    if (!kSplit && elect_one()) load_a(kb);
                 __syncwarp();
             }
             for (; ok && kb < kb1; ++kb, advance()) {
@@ -327,16 +339,17 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                 __syncwarp();
             }
         } else if (warp >= 8) {
-            const int rows = at.rows_here(), blocks = kb1 - kb0, turn = warp - 8;
-            // Piece i of this lane: elements 8 (lane % 16) .. of the K-block, of row 2 i + lane / 16.  (stage, phase: those of the item's first block)
-            const int row0 = lane / 16, chunk = lane % 16;
+            const int rows = at.rows_here(), blocks = kb1 - kb0, team = (warp - 8) / S::kTeam, member = (warp - 8) % S::kTeam;
+            // Piece i of this lane: elements 8 (lane % 16) .. of the K-block, of row 2 (i kTeam + member) + lane / 16.  (stage, phase: those of
+            // the item's first block)
+            const int row0 = member * 2 + lane / 16, chunk = lane % 16;
             uint32_t b_stage = stage, b_phase = phase;
             for (int b = 0; ok && b < blocks; ++b) {
                 const uint32_t at_stage = b_stage, at_phase = b_phase;
                 b_stage = b_stage + 1 == kStages ? 0 : b_stage + 1;
                 b_phase ^= b_stage == 0;
-                // (counted over all items: a warp is then never more than kSplitWarps blocks away from its last one)
-                if ((steps + b) % S::kSplitWarps != static_cast<uint32_t>(turn)) continue;
+                // (counted over all items: a team is then never more than kTeams blocks away from its last one)
+                if ((steps + b) % S::kTeams != static_cast<uint32_t>(team)) continue;
                 // First that the stage's block before this one has been multiplied, then that this one's A has landed.  Copies land in any
                 // order, and a warp that only asked for the latter could ask while the copy of the block before is still
                 // under way: a barrier two phases behind answers like one that is done.
@@ -347,8 +360,8 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                 uint8_t* const sf = smem + S::kOffSfb + at_stage * 512;
                 #pragma unroll
                 for (int i = 0; i < S::kPieces; ++i) {
-                    if (2 * i < rows) {                                      // (a row beyond the last one beside it: its columns are not stored)
-                        const int row = row0 + 2 * i, col = kTokens + row;
+                    if (2 * (S::kTeam * i + member) < rows) {                // (a row beyond the last one beside it: its columns are not stored)
+                        const int row = row0 + 2 * S::kTeam * i, col = kTokens + row;
                         uint2 hi, lo;
                         const uint32_t code = split_bf16(*reinterpret_cast<const uint4*>(a + row * 256), hi, lo);
                         const int to = (((chunk / 2) ^ (row & 7)) << 4) + chunk % 2 * 8;

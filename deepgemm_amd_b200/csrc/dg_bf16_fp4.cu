@@ -18,21 +18,21 @@ int run_split_a_gemm(const dg_gemm_args_t* args, bool ragged, int plane_rows);  
 
 namespace {
 
-// Clusters of S CTAs that run at once with two CTAs on an SM: what 148-SM B200s showed (a cluster lives inside one GPC, and a few SMs belong to
-// none that takes more than two)
-int clusters_at_once(int slices) {
-    static const int kFit[few::kMaxCluster + 1] = {0, 296, 148, 92, 70, 55, 44, 36, 31};
-    return std::max(1, kFit[slices] * dg_get_num_sms() / 148);
+// Clusters of S CTAs that run at once with one or two CTAs on an SM: what 148-SM B200s showed (a cluster lives inside one GPC, and a few SMs
+// belong to none that takes more than two)
+int clusters_at_once(int slices, int ctas_per_sm) {
+    static const int kFit[2][few::kMaxCluster + 1] = {{0, 148, 74, 45, 33, 26, 22, 15, 15}, {0, 296, 148, 93, 71, 56, 45, 36, 31}};
+    return std::max(1, kFit[ctas_per_sm - 1][slices] * dg_get_num_sms() / 148);
 }
 
-// CTAs along K (a cluster) for a launch with `items` blocks of 128 columns: the number with the fewest K-blocks in a row (~0.3 us each, an
+// CTAs along K (a cluster) for a launch with `items` blocks of 128 columns: the number with the fewest K-blocks in a row (~0.25 us each, an
 // SM's two CTAs side by side), a little more with partners, which finish an item before they begin the next
-int choose_slices(int64_t items, int num_blocks) {
+int choose_slices(int64_t items, int num_blocks, int ctas_per_sm) {
     int best = 1;
     double best_cost = 0.0;
     for (int s = 1; s <= few::kMaxCluster && (s == 1 || num_blocks / s >= 2); ++s) {
-        const double waves = static_cast<double>(ceil_div<int64_t>(items, clusters_at_once(s)));
-        const double cost = waves * (0.3 * ceil_div(num_blocks, s) + (s > 1 ? 1.5 : 0.0));
+        const double waves = static_cast<double>(ceil_div<int64_t>(items, clusters_at_once(s, ctas_per_sm)));
+        const double cost = waves * (0.25 * ceil_div(num_blocks, s) + (s > 1 ? 1.5 : 0.0));
         if (s == 1 || cost < best_cost) {
             best = s;
             best_cost = cost;
@@ -132,7 +132,7 @@ int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Plane
     // Items: exact for a dense product; a ragged one has at most one group per row, and a pass more per kTokens rows
     const int64_t tiles_n = ceil_div(g->n, 128), passes = ceil_div(g->m, kTokens);
     const int64_t items = tiles_n * (p.group_ends != nullptr ? std::min(g->m, g->num_groups + g->m / kTokens) : passes);
-    const int slices = choose_slices(items, g->k / 128);
+    const int slices = choose_slices(items, g->k / 128, S::kCtasPerSm);
     CUtensorMap tm_w, tm_sf, tm_a, tm_sfa;
     int rc;
     const uint64_t words = ceil_div(g->k, 4 * g->gran_k_b);
@@ -154,7 +154,7 @@ int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Plane
     const int smem = S::smem_bytes(slices);
     DG_CUDA_RT(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items, clusters_at_once(slices))) * slices);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items, clusters_at_once(slices, S::kCtasPerSm))) * slices);
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(g->stream);
@@ -165,7 +165,7 @@ int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Plane
         attrs[cfg.numAttrs].val.clusterDim.y = attrs[cfg.numAttrs].val.clusterDim.z = 1;
         ++cfg.numAttrs;
     }
-    if (state().pdl || !kSplit) {                // behind the kernel that splits A always: it lets this one start early
+    if (true) {                // behind the kernel that splits A always: it lets this one start early
         attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
@@ -190,7 +190,7 @@ int launch_many_rows(const dg_gemm_args_t* g, bool ragged, const Planes& planes)
 
 // Rows of A one product multiplies with a matrix of weights (ragged: on average; the sizes are on the device)
 int typical_rows(const dg_gemm_args_t* g, bool ragged) { return ragged ? ceil_div(g->m, g->num_groups) : g->m; }
-bool splits_inside(const dg_gemm_args_t* g, bool ragged) { return typical_rows(g, ragged) <= 8; }
+bool splits_inside(const dg_gemm_args_t* g, bool ragged) { return typical_rows(g, ragged) <= 16; }
 
 size_t workspace_bytes(const dg_gemm_args_t* g, bool ragged) {
     return g->m == 0 || g->n == 0 || splits_inside(g, ragged) ? 0 : planes_bytes(num_slots(g->m, g->num_groups, ragged), g->k);
@@ -227,9 +227,10 @@ int run(const dg_gemm_args_t* g, bool ragged, void* workspace, int64_t given_byt
     const Planes planes{static_cast<uint8_t*>(workspace), reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + static_cast<size_t>(2) * slots * g->k), slots};
     const Bf16Fp4Params p{g->d, ragged ? g->grouped_layout : nullptr, state().status_device, g->m, g->n, g->k, g->ldd, g->d_dtype == DG_FP32,
                           g->accumulate != 0, g->has_alpha ? g->alpha : 1.0f, slots, g->num_groups};
-    if (splits_inside(g, ragged)) return launch_few_rows<8, true>(g, p, planes);
-    if (rows <= 16) return launch_few_rows<16, false>(g, p, planes);
+    if (rows <= (ragged ? 4 : 8)) return launch_few_rows<8, true>(g, p, planes);
+    if (rows <= 16) return launch_few_rows<16, true>(g, p, planes);
     // (the GEMM kernel stores whole 16-byte pieces of a row of D: where N ends inside one, what follows the row would not stay)
+    if (rows > 32 && rows <= 64) return launch_few_rows<64, false>(g, p, planes);
     if (rows <= 32 || (static_cast<int64_t>(g->n) * d_elem) % 16 != 0) return launch_few_rows<32, false>(g, p, planes);
     return launch_many_rows(g, ragged, planes);
 }
