@@ -28,6 +28,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "ptx.cuh"
 #include "tile_scheduler.cuh"
 
@@ -55,37 +57,48 @@ __device__ __forceinline__ void group_rows(const Bf16Fp4Params& p, int g, int& f
     }
 }
 
-// One thread's share of the split: eight elements of a row, the four threads of an aligned quad holding 32 consecutive ones.
-// hi, lo: eight E4M3 values each; returns the UE8M0 code of hi's scale (lo's is 4 less), 255 (NaN) for a block with an infinity or NaN.
-__device__ __forceinline__ uint32_t split_bf16(const uint4& raw, uint2& hi, uint2& lo) {
-    const uint32_t x[4] = {raw.x, raw.y, raw.z, raw.w};
-    const uint32_t most2 = __vmaxu2(__vmaxu2(x[0] & 0x7FFF7FFFu, x[1] & 0x7FFF7FFFu), __vmaxu2(x[2] & 0x7FFF7FFFu, x[3] & 0x7FFF7FFFu));
-    uint32_t most = max(most2 & 0xFFFFu, most2 >> 16);                       // the bits of |x| order like |x|
-    most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-    most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-    // |x| = f 2^e with 448 = 1.75 2^8: the code of s is e - 8, one more when f > 1.75.  (Not below 4, so that lo has a code: a block
-    // whose largest element is below 2^-115 is then held to 2^-137)
-    const uint32_t code = max(static_cast<int>((most >> 7) + ((most & 0x7Fu) > 0x60u ? 1u : 0u)) - 8, 4);
-    const __nv_bfloat16 inv = __ushort_as_bfloat16(static_cast<unsigned short>((254u - code) << 7));       // 1 / s
-    uint32_t h[4], l[4];
+// One thread's share of the split: N pieces of eight elements of a row, the four threads of an aligned quad holding 32 consecutive ones.
+// hi, lo: eight E4M3 values each; code: UE8M0 code of hi's scale (lo's is 4 less), 255 (NaN) for a block with an infinity or NaN.
+template <int N>
+__device__ __forceinline__ void split_bf16(const uint4 (&raw)[N], uint2 (&hi)[N], uint2 (&lo)[N], uint32_t (&code)[N]) {
+    uint32_t most[N];
     #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x[i]), __halves2bfloat162(inv, inv));      // exact
-        const uint32_t bits = *reinterpret_cast<const uint32_t*>(&y);
-        const __half2 f = __floats2half2_rn(__uint_as_float(bits << 16), __uint_as_float(bits & 0xFFFF0000u));               // |y| <= 448: exact from 2^-17 on
-        uint16_t q;
-        uint32_t back;
-        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(q) : "r"(*reinterpret_cast<const uint32_t*>(&f)));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(q));
-        const __half2 rest = __hmul2(__hsub2(f, *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(16.0f));
-        uint16_t r;
-        asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
-        h[i] = q;
-        l[i] = r;
+    for (int p = 0; p < N; ++p) {
+        const uint4& x = raw[p];
+        const uint32_t most2 = __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
+        most[p] = max(most2 & 0xFFFFu, most2 >> 16);                         // the bits of |x| order like |x|
     }
-    hi = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-    lo = make_uint2(l[0] | (l[1] << 16), l[2] | (l[3] << 16));
-    return most >= 0x7F80u ? 255u : code;
+    #pragma unroll
+    for (int p = 0; p < N; ++p) most[p] = max(most[p], __shfl_xor_sync(0xFFFFFFFFu, most[p], 1));
+    #pragma unroll
+    for (int p = 0; p < N; ++p) most[p] = max(most[p], __shfl_xor_sync(0xFFFFFFFFu, most[p], 2));
+    #pragma unroll
+    for (int p = 0; p < N; ++p) {
+        const uint32_t x[4] = {raw[p].x, raw[p].y, raw[p].z, raw[p].w};
+        // |x| = f 2^e with 448 = 1.75 2^8: the code of s is e - 8, one more when f > 1.75.  (Not below 4, so that lo has a code: a block
+        // whose largest element is below 2^-115 is then held to 2^-137)
+        const uint32_t c = max(static_cast<int>((most[p] >> 7) + ((most[p] & 0x7Fu) > 0x60u ? 1u : 0u)) - 8, 4);
+        const __nv_bfloat16 inv = __ushort_as_bfloat16(static_cast<unsigned short>((254u - c) << 7));      // 1 / s
+        uint32_t h[4], l[4];
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x[i]), __halves2bfloat162(inv, inv));  // exact
+            const uint32_t bits = *reinterpret_cast<const uint32_t*>(&y);
+            const __half2 f = __floats2half2_rn(__uint_as_float(bits << 16), __uint_as_float(bits & 0xFFFF0000u));           // |y| <= 448: exact from 2^-17 on
+            uint16_t q;
+            uint32_t back;
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(q) : "r"(*reinterpret_cast<const uint32_t*>(&f)));
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(q));
+            const __half2 rest = __hmul2(__hsub2(f, *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(16.0f));
+            uint16_t r;
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
+            h[i] = q;
+            l[i] = r;
+        }
+        hi[p] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+        lo[p] = make_uint2(l[0] | (l[1] << 16), l[2] | (l[3] << 16));
+        code[p] = most[p] >= 0x7F80u ? 255u : c;
+    }
 }
 
 namespace few {
@@ -165,8 +178,8 @@ template <int kTokens, bool kSplit> struct Shape {
     static constexpr int kCols = 2 * kTokens;                                // columns of the tile
     static constexpr int kStages = kTokens == 8 ? 5 : (kTokens == 16 ? 4 : (kTokens == 32 ? 3 : 5)), kCtasPerSm = kTokens <= 32 ? 2 : 1;
     // Teams of splitting warps take turns at the K-blocks: a block's chain of wait, shuffles, conversions, stores and fence is long, so as
-    // many blocks as possible are at it at once.  Every lane splits four pieces of eight elements of a block
-    static constexpr int kTeams = 4, kTeam = kTokens / 8, kPieces = 4, kSplitWarps = kTeams * kTeam;
+    // many blocks as possible are at it at once
+    static constexpr int kTeams = 4, kTeam = 2, kPieces = kTokens / (2 * kTeam), kSplitWarps = kTeams * kTeam;
     static constexpr int kThreads = kSplit ? 256 + 32 * kSplitWarps : 256;
     static_assert(!kSplit || (kTokens <= 16 && kTeams <= kStages), "a team that is done with its last block knows that the stage of its next one is at most one block behind");
     static constexpr int kOffB = kStages * 16384, kOffA = kOffB + kStages * kCols * 128, kOffSfa = kOffA + (kSplit ? kStages * kTokens * 256 : 0), kOffSfb = kOffSfa + kStages * 512;
@@ -358,21 +371,31 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                 const uint8_t* const a = smem + S::kOffA + at_stage * kTokens * 256 + chunk * 16;
                 uint8_t* const tile = smem + S::kOffB + at_stage * kCols * 128;
                 uint8_t* const sf = smem + S::kOffSfb + at_stage * 512;
-                #pragma unroll
-                for (int i = 0; i < S::kPieces; ++i) {
-                    if (2 * (S::kTeam * i + member) < rows) {                // (a row beyond the last one beside it: its columns are not stored)
+                // (pieces side by side, so that their chains of shuffles and conversions overlap; rows beyond the last one are split along with
+                // the others: their columns are not stored)
+                auto split = [&](auto pieces) {
+                    constexpr int kN = decltype(pieces)::value;
+                    uint4 raw[kN];
+                    uint2 hi[kN], lo[kN];
+                    uint32_t code[kN];
+                    #pragma unroll
+                    for (int i = 0; i < kN; ++i) raw[i] = *reinterpret_cast<const uint4*>(a + (row0 + 2 * S::kTeam * i) * 256);
+                    split_bf16<kN>(raw, hi, lo, code);
+                    #pragma unroll
+                    for (int i = 0; i < kN; ++i) {
                         const int row = row0 + 2 * S::kTeam * i, col = kTokens + row;
-                        uint2 hi, lo;
-                        const uint32_t code = split_bf16(*reinterpret_cast<const uint4*>(a + row * 256), hi, lo);
                         const int to = (((chunk / 2) ^ (row & 7)) << 4) + chunk % 2 * 8;
-                        *reinterpret_cast<uint2*>(tile + row * 128 + to) = hi;
-                        *reinterpret_cast<uint2*>(tile + col * 128 + to) = lo;
+                        *reinterpret_cast<uint2*>(tile + row * 128 + to) = hi[i];
+                        *reinterpret_cast<uint2*>(tile + col * 128 + to) = lo[i];
                         if (chunk % 4 == 0) {
-                            sf[row * 16 + chunk / 4] = static_cast<uint8_t>(code);
-                            sf[col * 16 + chunk / 4] = static_cast<uint8_t>(code == 255 ? 255 : code - 4);
+                            sf[row * 16 + chunk / 4] = static_cast<uint8_t>(code[i]);
+                            sf[col * 16 + chunk / 4] = static_cast<uint8_t>(code[i] == 255 ? 255 : code[i] - 4);
                         }
                     }
-                }
+                };
+                if (S::kPieces == 1 || rows <= 2 * S::kTeam) split(std::integral_constant<int, 1>{});
+                else if (S::kPieces == 2 || rows <= 4 * S::kTeam) split(std::integral_constant<int, (S::kPieces < 2 ? 1 : 2)>{});
+                else split(std::integral_constant<int, S::kPieces>{});
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full_bar(at_stage));

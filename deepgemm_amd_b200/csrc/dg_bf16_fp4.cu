@@ -59,6 +59,8 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* __
                                                          const int* __restrict__ group_ends, int groups) {
     __shared__ int slot_of[kSplitRows];
     __shared__ uint32_t words[2][kSplitCols / 128][kSplitRows];
+    // (in this order: what the product's kernel reads before it waits for this one, the weights, is then complete as well)
+    griddep_wait();
     griddep_launch_dependents();
     const int row0 = blockIdx.y * kSplitRows, r = threadIdx.x / 16, chunk = threadIdx.x % 16, row = row0 + r;
     if (threadIdx.x < kSplitRows) {
@@ -86,16 +88,17 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* __
         raw[b] = make_uint4(0, 0, 0, 0);
         if (slot >= 0 && col < k) raw[b] = __ldg(reinterpret_cast<const uint4*>(a + row * lda + col));
     }
+    uint2 hi[kSplitCols / 128], lo[kSplitCols / 128];
+    uint32_t code[kSplitCols / 128];
+    split_bf16<kSplitCols / 128>(raw, hi, lo, code);
     #pragma unroll
     for (int b = 0; b < kSplitCols / 128; ++b) {
         const int col = blockIdx.x * kSplitCols + b * 128 + chunk * 8;
-        uint2 hi, lo;
-        const uint32_t code = split_bf16(raw[b], hi, lo);
         if (slot >= 0 && col < k) {
-            *reinterpret_cast<uint2*>(out.q + static_cast<int64_t>(slot) * k + col) = hi;
-            *reinterpret_cast<uint2*>(out.q + (static_cast<int64_t>(out.slots) + slot) * k + col) = lo;
+            *reinterpret_cast<uint2*>(out.q + static_cast<int64_t>(slot) * k + col) = hi[b];
+            *reinterpret_cast<uint2*>(out.q + (static_cast<int64_t>(out.slots) + slot) * k + col) = lo[b];
         }
-        uint32_t word = code << (chunk / 4 * 8);
+        uint32_t word = code[b] << (chunk / 4 * 8);
         word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
         word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
         if (chunk == 0) {
@@ -120,9 +123,16 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* __
 
 int split_rows(const dg_gemm_args_t* g, const int* group_ends, const Planes& planes) {
     const dim3 grid(ceil_div(g->k, kSplitCols), ceil_div(g->m, kSplitRows));
-    split_rows_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(g->stream)>>>(static_cast<const __nv_bfloat16*>(g->a), g->lda, planes, g->m, g->k, group_ends,
-                                                                               g->num_groups);
-    DG_CUDA_RT(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(256);
+    cfg.stream = static_cast<cudaStream_t>(g->stream);
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    DG_CUDA_RT(cudaLaunchKernelEx(&cfg, split_rows_kernel, static_cast<const __nv_bfloat16*>(g->a), g->lda, planes, g->m, g->k, group_ends, g->num_groups));
     return DG_OK;
 }
 
@@ -165,10 +175,10 @@ int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Plane
         attrs[cfg.numAttrs].val.clusterDim.y = attrs[cfg.numAttrs].val.clusterDim.z = 1;
         ++cfg.numAttrs;
     }
-    if (true) {                // behind the kernel that splits A always: it lets this one start early
-        attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    }
+    // Always launched behind its predecessor's start rather than its end: it waits for that kernel itself, before it reads anything that one
+    // may have written, and has set up by then (2 us of a token's 6 through N 2112 K 7168)
+    attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attrs;
     DG_CUDA_RT(cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_sf, tm_a, tm_sfa, p));
     return DG_OK;
@@ -188,9 +198,28 @@ int launch_many_rows(const dg_gemm_args_t* g, bool ragged, const Planes& planes)
     return run_split_a_gemm(&args, ragged, planes.slots);
 }
 
-// Rows of A one product multiplies with a matrix of weights (ragged: on average; the sizes are on the device)
-int typical_rows(const dg_gemm_args_t* g, bool ragged) { return ragged ? ceil_div(g->m, g->num_groups) : g->m; }
-bool splits_inside(const dg_gemm_args_t* g, bool ragged) { return typical_rows(g, ragged) <= 16; }
+// Which kernels a product takes, by the rows of A that meet one matrix of weights (ragged: on average; the sizes are on the device):
+//   up to 8      the few-row kernel, splitting A itself
+//   up to 16     the same with 16 rows a pass, as long as an SM has no more than ~16 blocks of 128 x 128 weights to go through; with more of them
+//                splitting A for each costs more than a kernel that splits it once (N 7168 K 16384: 26 us against 21; N 4096 K 7168: 10.5 against 11.4)
+//   up to 32     the few-row kernel on A split ahead
+//   above        the GEMM kernel on A split ahead (N 7168 K 2048: 11.4 us at 64 rows, the few-row kernel 13.3)
+enum class Form { kSplit8, kSplit16, kPlanes16, kPlanes32, kMany };
+Form form_of(const dg_gemm_args_t* g, bool ragged) {
+    const int rows = ragged ? ceil_div(g->m, g->num_groups) : g->m;
+    if (rows <= 8) return Form::kSplit8;
+    if (rows <= 16) {
+        const int64_t blocks = static_cast<int64_t>(ceil_div(g->n, 128)) * ceil_div(g->k, 128) * (ragged ? std::min(g->num_groups, g->m) : 1);
+        return blocks <= static_cast<int64_t>(16) * dg_get_num_sms() ? Form::kSplit16 : Form::kPlanes16;
+    }
+    // (the GEMM kernel stores whole 16-byte pieces of a row of D: where N ends inside one, what follows the row would not stay)
+    const int d_elem = g->d_dtype == DG_FP32 ? 4 : 2;
+    return rows <= 32 || (static_cast<int64_t>(g->n) * d_elem) % 16 != 0 ? Form::kPlanes32 : Form::kMany;
+}
+bool splits_inside(const dg_gemm_args_t* g, bool ragged) {
+    const Form form = form_of(g, ragged);
+    return form == Form::kSplit8 || form == Form::kSplit16;
+}
 
 size_t workspace_bytes(const dg_gemm_args_t* g, bool ragged) {
     return g->m == 0 || g->n == 0 || splits_inside(g, ragged) ? 0 : planes_bytes(num_slots(g->m, g->num_groups, ragged), g->k);
@@ -223,15 +252,17 @@ int run(const dg_gemm_args_t* g, bool ragged, void* workspace, int64_t given_byt
     DG_REQUIRE(needed == 0 || (workspace != nullptr && aligned(workspace, 128) && given_bytes >= 0 && static_cast<size_t>(given_bytes) >= needed));
     int rc = ensure_status_word();
     if (rc != DG_OK) return rc;
-    const int slots = num_slots(g->m, g->num_groups, ragged), rows = typical_rows(g, ragged);
+    const int slots = num_slots(g->m, g->num_groups, ragged);
     const Planes planes{static_cast<uint8_t*>(workspace), reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + static_cast<size_t>(2) * slots * g->k), slots};
     const Bf16Fp4Params p{g->d, ragged ? g->grouped_layout : nullptr, state().status_device, g->m, g->n, g->k, g->ldd, g->d_dtype == DG_FP32,
                           g->accumulate != 0, g->has_alpha ? g->alpha : 1.0f, slots, g->num_groups};
-    if (rows <= (ragged ? 4 : 8)) return launch_few_rows<8, true>(g, p, planes);
-    if (rows <= 16) return launch_few_rows<16, true>(g, p, planes);
-    // (the GEMM kernel stores whole 16-byte pieces of a row of D: where N ends inside one, what follows the row would not stay)
-    if (rows > 32 && rows <= 64) return launch_few_rows<64, false>(g, p, planes);
-    if (rows <= 32 || (static_cast<int64_t>(g->n) * d_elem) % 16 != 0) return launch_few_rows<32, false>(g, p, planes);
+    switch (form_of(g, ragged)) {
+        case Form::kSplit8: return launch_few_rows<8, true>(g, p, planes);
+        case Form::kSplit16: return launch_few_rows<16, true>(g, p, planes);
+        case Form::kPlanes16: return launch_few_rows<16, false>(g, p, planes);
+        case Form::kPlanes32: return launch_few_rows<32, false>(g, p, planes);
+        case Form::kMany: break;
+    }
     return launch_many_rows(g, ragged, planes);
 }
 
