@@ -1175,11 +1175,12 @@ m_grouped_fp4_gemm_nt_masked = m_grouped_fp8_fp4_gemm_nt_masked
 # ------------------------------------------------------------------------------------------------
 def get_gemm_config(kind: int, m: int, n: int, k: int, num_groups: int = 1, expected_m: int = 0,
                     b_is_fp4: bool = False, d_is_fp32: bool = False, gran_k_a: int = 128, gran_k_b: int = 128,
-                    d_is_fp8: bool = False, a_is_fp4: bool = False) -> dict:
-    """The tile configuration the heuristics choose for a problem (host only, needs no GPU)."""
+                    d_is_fp8: bool = False, a_is_fp4: bool = False, a_is_bf16: bool = False) -> dict:
+    """The tile configuration the heuristics choose for a problem (host only, needs no GPU).  a_is_bf16 with b_is_fp4: the
+    many-row form of the BF16 x FP4 products."""
     args = GemmArgs()
     args.m, args.n, args.k, args.num_groups = m, n, k, num_groups
-    args.a_dtype = _lib.DG_FP4_E2M1_X2 if a_is_fp4 else _lib.DG_FP8_E4M3
+    args.a_dtype = _lib.DG_BF16 if a_is_bf16 else (_lib.DG_FP4_E2M1_X2 if a_is_fp4 else _lib.DG_FP8_E4M3)
     args.b_dtype = _lib.DG_FP4_E2M1_X2 if b_is_fp4 else _lib.DG_FP8_E4M3
     args.d_dtype = _lib.DG_FP32 if d_is_fp32 else (_lib.DG_FP8_E4M3 if d_is_fp8 else _lib.DG_BF16)
     args.sfd_pitch = align(m, 4)
@@ -1194,11 +1195,12 @@ def get_gemm_config(kind: int, m: int, n: int, k: int, num_groups: int = 1, expe
 
 def precompile_gemm(kind: int, m: int, n: int, k: int, num_groups: int = 1, expected_m: int = 0,
                     b_is_fp4: bool = False, d_is_fp32: bool = False, accumulate: bool = False,
-                    gran_k_a: int = 128, gran_k_b: int = 128, d_is_fp8: bool = False, a_is_fp4: bool = False) -> None:
+                    gran_k_a: int = 128, gran_k_b: int = 128, d_is_fp8: bool = False, a_is_fp4: bool = False,
+                    a_is_bf16: bool = False) -> None:
     """Compile the kernel a GEMM of this shape would use into the cache (needs nvcc, no GPU)."""
     args = GemmArgs()
     args.m, args.n, args.k, args.num_groups = m, n, k, num_groups
-    args.a_dtype = _lib.DG_FP4_E2M1_X2 if a_is_fp4 else _lib.DG_FP8_E4M3
+    args.a_dtype = _lib.DG_BF16 if a_is_bf16 else (_lib.DG_FP4_E2M1_X2 if a_is_fp4 else _lib.DG_FP8_E4M3)
     args.b_dtype = _lib.DG_FP4_E2M1_X2 if b_is_fp4 else _lib.DG_FP8_E4M3
     args.d_dtype = _lib.DG_FP32 if d_is_fp32 else (_lib.DG_FP8_E4M3 if d_is_fp8 else _lib.DG_BF16)
     args.sfd_pitch = align(m, 4)

@@ -17,9 +17,9 @@
 //   warp 1      MMA issuer
 //   warp 2      allocates tensor memory, rearranges scale words for tcgen05.cp
 //   warps 4-7   epilogue
-//   warps 8-11  split the stage's rows of A into its tile columns and their scales (up to eight rows).  From nine rows on splitting them
-// again in every CTA costs more than the weights (a block of 32 rows took 0.6 us), so a kernel of its own does it once and this one loads the
-// two planes; it asks for the first stages of W before that kernel is done.
+//   warps 8-15  in teams of two: split a stage's rows of A into its tile columns and their scales.  For more rows, or more weights to a
+// CTA, splitting them again in every CTA costs more than the weights (a block of 16 rows takes a CTA 0.3 us, one of 32 0.6): a kernel of its own
+// then does it once and this one, without those warps, loads the two planes; it asks for the first stages of W before that kernel is done.
 // Where the items alone do not occupy the GPU, the CTAs of a cluster (up to 8) share an item's K and send their partial sums to one another
 // through distributed shared memory, every CTA adding up its own rows of D in rank order.  One CTA's ring of stages takes ~1.5 us to go
 // round (load, split, multiply), 0.3 us per block of 8 KB; two CTAs share an SM, which together ask for what HBM delivers.
@@ -173,10 +173,10 @@ struct Items {
     __device__ __forceinline__ int rows_here() const { return min(tokens, first + rows - row); }
 };
 
-// kSplit: the kernel splits A itself (a token or a few); otherwise A comes as the two planes of a kernel before this one
+// kSplit: the kernel splits A itself; otherwise A comes as the two planes of a kernel before this one
 template <int kTokens, bool kSplit> struct Shape {
     static constexpr int kCols = 2 * kTokens;                                // columns of the tile
-    static constexpr int kStages = kTokens == 8 ? 5 : (kTokens == 16 ? 4 : (kTokens == 32 ? 3 : 5)), kCtasPerSm = kTokens <= 32 ? 2 : 1;
+    static constexpr int kStages = kTokens == 8 ? 5 : (kTokens == 16 ? 4 : 3);      // two CTAs share an SM's 227 KB
     // Teams of splitting warps take turns at the K-blocks: a block's chain of wait, shuffles, conversions, stores and fence is long, so as
     // many blocks as possible are at it at once
     static constexpr int kTeams = 4, kTeam = 2, kPieces = kTokens / (2 * kTeam), kSplitWarps = kTeams * kTeam;
@@ -184,7 +184,8 @@ template <int kTokens, bool kSplit> struct Shape {
     static_assert(!kSplit || (kTokens <= 16 && kTeams <= kStages), "a team that is done with its last block knows that the stage of its next one is at most one block behind");
     static constexpr int kOffB = kStages * 16384, kOffA = kOffB + kStages * kCols * 128, kOffSfa = kOffA + (kSplit ? kStages * kTokens * 256 : 0), kOffSfb = kOffSfa + kStages * 512;
     static constexpr int kOffBar = kOffSfb + kStages * 512, kOffMisc = kOffBar + (4 * kStages + 4) * 8, kOffRecv = (kOffMisc + 8 + 15) / 16 * 16;
-    static constexpr int kTmemCols = 2 * kCols + 8 <= 64 ? 64 : (2 * kCols + 8 <= 128 ? 128 : (2 * kCols + 8 <= 256 ? 256 : 512));
+    static constexpr int kTmemCols = 2 * kCols + 8 <= 64 ? 64 : (2 * kCols + 8 <= 128 ? 128 : 256);
+    static_assert(kTokens <= 32, "two CTAs' shares of an SM's shared and tensor memory");
     // What a CTA receives: every slice's partial sums of the rows of D it owns
     __host__ __device__ static constexpr int recv_rows(int slices) { return (kTokens + slices - 1) / slices; }
     __host__ __device__ static constexpr int smem_bytes(int slices) { return kOffRecv + (slices > 1 ? slices * recv_rows(slices) * 512 : 0); }
@@ -192,7 +193,7 @@ template <int kTokens, bool kSplit> struct Shape {
 
 // kGran: elements of K per scale of W
 template <int kTokens, bool kSplit, int kGran>
-__global__ void __launch_bounds__(Shape<kTokens, kSplit>::kThreads, Shape<kTokens, kSplit>::kCtasPerSm)
+__global__ void __launch_bounds__(Shape<kTokens, kSplit>::kThreads, 2)
 bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_sf, const __grid_constant__ CUtensorMap tm_a,
                          const __grid_constant__ CUtensorMap tm_sfa, const Bf16Fp4Params p) {
     using S = Shape<kTokens, kSplit>;

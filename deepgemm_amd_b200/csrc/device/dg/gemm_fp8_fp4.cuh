@@ -45,7 +45,8 @@
 //
 // DG_PLANES == 2: A is a BF16 matrix split into two E4M3 matrices, A = hi + lo with a scale per 32 elements of K each (dg_bf16_fp4.cu), and
 // the product is hi B^T + lo B^T: a stage holds 128 rows of either and one B, which both MMAs of a K-block read into one accumulator.  Two
-// E4M3 x E2M1 MMAs take the time of one in BF16, without B ever being widened.
+// E4M3 x E2M1 MMAs take the time of one in BF16, without B ever being widened.  A tile of which at most 64 rows count ("half": a small group, or
+// the end of one) is one MMA instead of two: hi's 64 rows above lo's in one 128-row operand, added up in the epilogue.
 //
 // ragged (type 6): groups of rows of any size follow one another in D without padding; the rows of A lie in slots (tile_scheduler.cuh).
 //
@@ -148,6 +149,7 @@ constexpr uint32_t kL2Hint     = DG_L2_HINT;
 #define DG_PLANES 1
 #endif
 constexpr uint32_t kPlanes     = DG_PLANES;        // E4M3 matrices that make up A
+constexpr bool     kHalfTiles  = kPlanes == 2 && kCluster == 1;
 
 constexpr uint32_t UMMA_M = 128 * kCluster, UMMA_N = BLOCK_N, UMMA_K = 32;
 constexpr uint32_t LOAD_BLOCK_N = BLOCK_N / kCluster;      // rows of B each CTA loads
@@ -255,6 +257,7 @@ constexpr uint32_t kGroupCols       = kLayout.group_cols();          // columns 
 constexpr uint32_t kNumGroups       = kLayout.num_groups();
 constexpr uint32_t kNumStoreStages  = kLayout.num_store_stages();
 constexpr uint32_t kStoreStageBytes = kLayout.store_stage_bytes();
+static_assert(!kHalfTiles || kGroupCols * 64 * 4 <= kStoreStageBytes, "half tiles: 64 rows of a group in FP32 fit a staging buffer");
 constexpr uint32_t kSmemD   = kLayout.off_d();
 constexpr uint32_t kSmemA   = kLayout.off_a();
 // Cluster-reduced K slicing: columns of the tile a CTA owns (whole 8-column chunks, dealt round robin), and the bytes it
@@ -468,6 +471,11 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
     // A 256-row tile of the contiguous layout whose halves belong to different experts takes two passes over K:
     // pass h multiplies half h with B of its own expert
     auto num_passes_of = [&](const Tile& t) { return kGemmType == 1 && kMHalves == 2 && t.group1 != t.group ? 2u : 1u; };
+    // Split A: whether the tile has at most 64 rows that count
+    auto is_half = [&](const Tile& t) {
+        if constexpr (!kHalfTiles) return false;
+        return (kGemmType == kDense ? p.shape_m - t.m_block * TILE_M : t.valid_rows) <= 64;
+    };
     // Every role walks the same sequence of (pass, K-block) steps of a tile, one pipeline stage per step
     struct Step { uint32_t pass, kb; };
     auto step_of = [](uint32_t it, uint32_t kb0, uint32_t num_kb) {
@@ -540,21 +548,24 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                         DG_PROF_ADD(prof_wait, prof_w);
                         if constexpr (kProducerWholeWarp) __syncwarp();
                         if (kProducerWholeWarp && lane != 0) { advance_sf(kb); continue; }
+                        [[maybe_unused]] const bool half = is_half(tile);
                         if constexpr (kHasSF) {
                             uint32_t sf_bytes = 0;
-                            if (kb % kSFAPeriod == 0) sf_bytes += kSFABytes;
+                            if (kb % kSFAPeriod == 0) sf_bytes += half ? kSFABytes / 2 : kSFABytes;
                             if (kb % kSFBPeriod == 0) sf_bytes += kSFBBytes;
                             mbar_arrive_expect_tx(sf_full_bar(stage), sf_bytes);
                             if (kb % kSFAPeriod == 0)
                                 // (split A: the two planes' words of a K-block are two rows, one box)
                                 tma_in(sfa_buffer(), &tm_sfa, sf_full_bar(stage), sfa_mn, sfa_row0 + kb / kSFAPeriod * kSFAWords * kPlanes, tile.group);
+                            if (kHalfTiles && kb % kSFAPeriod == 0 && !half)       // (boxes of 64 rows)
+                                tma_in(sfa_buffer() + kSFABytes / 2, &tm_sfa, sf_full_bar(stage), sfa_mn + 64, sfa_row0 + kb / kSFAPeriod * kSFAWords * kPlanes, tile.group);
                             if (kb % kSFBPeriod == 0)
                                 tma_in(sfb_buffer(), &tm_sfb, sf_full_bar(stage), tile.n_block * BLOCK_N, sfb_row0 + kb / kSFBPeriod * kSFBWords, tile.group);
                         }
                         // With a cluster the copies land in this CTA and their bytes are counted on CTA 0's barrier,
                         // which expects both CTAs' bytes
                         const uint32_t load_bar = kCluster == 1 ? full_bar(stage) : in_leader(full_bar(stage));
-                        if (kCluster == 1 || is_leader) mbar_arrive_expect_tx(full_bar(stage), kTxBytesAB);
+                        if (kCluster == 1 || is_leader) mbar_arrive_expect_tx(full_bar(stage), kTxBytesAB - (half ? kABytes / 2 : 0u));
                         else mbar_arrive_cluster(load_bar);
                         auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y) {
                             if constexpr (kL2Hint != 0 && kGemmType != kBatched) {
@@ -582,8 +593,17 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                             #pragma unroll
                             for (uint32_t ka = 0; ka < kKAtoms; ++ka)       // one box of the stage's rows per 128 bytes of K
                                 load(smem_base + kSmemA + stage * kABytes + ka * kAAtomStride, &tm_a, k_base + kb * kLoadXPerKBlock + ka * 128, a_row);
-                            if constexpr (kPlanes == 2)
+                            if constexpr (kHalfTiles) {
+                                // boxes of 64 rows: hi's, then lo's of a half tile; hi's two and lo's two of a whole one (the first is on its way)
+                                const uint32_t a_stage = smem_base + kSmemA + stage * kABytes, kx = kb * kLoadXPerKBlock;
+                                load(a_stage + 64 * BLOCK_K, &tm_a, kx, half ? p.plane_rows + a_row : a_row + 64);
+                                if (!half) {
+                                    load(a_stage + 128 * BLOCK_K, &tm_a, kx, p.plane_rows + a_row);
+                                    load(a_stage + 192 * BLOCK_K, &tm_a, kx, p.plane_rows + a_row + 64);
+                                }
+                            } else if constexpr (kPlanes == 2) {
                                 load(smem_base + kSmemA + stage * kABytes + kABytes / 2, &tm_a, k_base + kb * kLoadXPerKBlock, p.plane_rows + a_row);
+                            }
                         } else {
                             // one box per atom: 128 bytes of M (128 FP8 or 64 BF16 elements) by the stage's rows of K
                             #pragma unroll
@@ -663,6 +683,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                     tc_fence_after_sync();
                     const uint32_t kb0 = kb_begin(tile), num_kb = kb_end(tile) - kb0;
                     const uint32_t num_passes = num_passes_of(tile), num_steps = num_passes * num_kb;
+                    [[maybe_unused]] const bool half = is_half(tile);
                     for (uint32_t it = 0; it < num_steps; ++it, advance_stage()) {
                         const auto [pass, kb] = step_of(it, kb0, num_kb);
                         DG_PROF_BEGIN(prof_w1);
@@ -679,7 +700,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                         if (kHasSF && kb % kSFAPeriod == 0) {
                             #pragma unroll
                             for (uint32_t i = 0; i < kSFAWords * SF_BLOCK_M / 128 * kPlanes; ++i)      // chunk (word w, rows 128 r ..): index w * (rows / 128) + r
-                                tc_cp_32x128b_warpx4<kCluster>(tmem_base + kTmemColSFA + i * 4,
+                                if (!(half && i > 0)) tc_cp_32x128b_warpx4<kCluster>(tmem_base + kTmemColSFA + i * 4,
                                                                make_smem_desc(sfa_buffer() + i * 512, 0, 128, kSwizzleNone));
                         }
                         if (kHasSF && kb % kSFBPeriod == 0) {
@@ -696,6 +717,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                         for (uint32_t pl = 0; pl < kPlanes; ++pl)
                         #pragma unroll
                         for (uint32_t h = 0; h < kMHalves; ++h) {
+                            if (half && pl > 0) continue;
                             // In a two-pass tile (halves of different experts) pass p carries half p's expert
                             if (num_passes == 2 && h != pass) continue;
                             // Half h: rows [128 h, 128 h + 128) of the A stage (128 * BLOCK_K bytes further, in either layout),
@@ -767,14 +789,26 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
             DG_PROF_BEGIN(prof_t0);
             while (ok && sched.next(tile)) {
                 const uint32_t kb0 = kb_begin(tile), num_kb = kb_end(tile) - kb0, num_steps = num_passes_of(tile) * num_kb;
+                [[maybe_unused]] const bool half = is_half(tile);
                 for (uint32_t it = 0; it < num_steps; ++it, advance_stage()) {
                     const uint32_t kb = step_of(it, kb0, num_kb).kb;
                     DG_PROF_BEGIN(prof_w);
                     if (!mbar_wait(sf_full_bar(stage), phase, ctx, kRoleSF, 1)) { ok = false; break; }
                     DG_PROF_ADD(prof_wait, prof_w);
-                    if (kb % kSFAPeriod == 0) {
+                    if (kHalfTiles && kb % kSFAPeriod == 0 && !half) {
+                        // two boxes of [hi, lo][64 rows]: gather the planes' 128 rows each on the way
+                        uint32_t v[2][4];
                         #pragma unroll
-                        for (uint32_t i = 0; i < kSFAWords * SF_BLOCK_M / 128 * kPlanes; ++i)
+                        for (uint32_t pl = 0; pl < 2; ++pl)
+                            #pragma unroll
+                            for (uint32_t c = 0; c < 4; ++c)
+                                v[pl][c] = ld_shared_u32(sfa_buffer() + c / 2 * 512 + pl * 256 + (c % 2 * 32 + lane) * 4);
+                        __syncwarp();
+                        #pragma unroll
+                        for (uint32_t pl = 0; pl < 2; ++pl) st_shared_v4(sfa_buffer() + pl * 512 + lane * 16, v[pl][0], v[pl][1], v[pl][2], v[pl][3]);
+                    } else if (kb % kSFAPeriod == 0) {
+                        #pragma unroll
+                        for (uint32_t i = 0; i < (kHalfTiles ? 1 : kSFAWords * SF_BLOCK_M / 128 * kPlanes); ++i)
                             rearrange(sfa_buffer() + i * 512);
                     }
                     if (kb % kSFBPeriod == 0) {
@@ -971,6 +1005,11 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                                 #pragma unroll
                                 for (uint32_t r = 0; r < kSplitCluster; ++r)
                                     sum[i] += __uint_as_float(ld_shared_u32(recv + ((r * kRecvCols + jj * 8 + i) * BLOCK_M + row_in_tile) * 4));
+                                if (kHalfTiles && is_half(tile)) {                  // (rows that count are below 64: lo's are 64 further down)
+                                    #pragma unroll
+                                    for (uint32_t r = 0; r < kSplitCluster; ++r)
+                                        sum[i] += __uint_as_float(ld_shared_u32(recv + ((r * kRecvCols + jj * 8 + i) * BLOCK_M + row_in_tile % 64 + 64) * 4));
+                                }
                                 sum[i] *= p.alpha;
                             }
                             if constexpr (kDIsFP32) {
@@ -1110,6 +1149,27 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                             for (uint32_t i = 0; i < 16; ++i)
                                 v[l][i] = __float_as_uint(__uint_as_float(v[l][i]) * p.alpha);
                         }
+                }
+                if constexpr (kHalfTiles) {
+                    if (is_half(tile)) {
+                        // Lanes 64 .. 127 hold lo's products of rows 0 .. 63: through a staging buffer (column by column, so that a warp's
+                        // rows are neighbours) to the lanes that hold hi's
+                        if (epi_tid == 0) tma_store_wait_read<0>();
+                        named_barrier_sync(bar_id, kNumEpilogueThreads);
+                        if (row_in_tile >= 64) {
+                            #pragma unroll
+                            for (uint32_t c = 0; c < kGroupCols; ++c)
+                                if (c < kCols) st_shared_u32(staging + (c * 64 + row_in_tile - 64) * 4, v[c / 16][c % 16]);
+                        }
+                        named_barrier_sync(bar_id, kNumEpilogueThreads);
+                        if (row_in_tile < 64) {
+                            #pragma unroll
+                            for (uint32_t c = 0; c < kGroupCols; ++c)
+                                if (c < kCols) v[c / 16][c % 16] = __float_as_uint(__uint_as_float(v[c / 16][c % 16]) +
+                                                                                   __uint_as_float(ld_shared_u32(staging + (c * 64 + row_in_tile) * 4)));
+                        }
+                        named_barrier_sync(bar_id, kNumEpilogueThreads);
+                    }
                 }
                 // Quantised output: the group's BF16-rounded values, 32 columns per scale, as e4m3 words; the scale bytes
                 // go straight to global memory (one byte per row and 32 columns)

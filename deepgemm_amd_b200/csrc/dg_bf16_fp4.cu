@@ -18,20 +18,20 @@ int run_split_a_gemm(const dg_gemm_args_t* args, bool ragged, int plane_rows);  
 
 namespace {
 
-// Clusters of S CTAs that run at once with one or two CTAs on an SM: what 148-SM B200s showed (a cluster lives inside one GPC, and a few SMs
+// Clusters of S CTAs that run at once with two CTAs on an SM: what 148-SM B200s showed (a cluster lives inside one GPC, and a few SMs
 // belong to none that takes more than two)
-int clusters_at_once(int slices, int ctas_per_sm) {
-    static const int kFit[2][few::kMaxCluster + 1] = {{0, 148, 74, 45, 33, 26, 22, 15, 15}, {0, 296, 148, 93, 71, 56, 45, 36, 31}};
-    return std::max(1, kFit[ctas_per_sm - 1][slices] * dg_get_num_sms() / 148);
+int clusters_at_once(int slices) {
+    static const int kFit[few::kMaxCluster + 1] = {0, 296, 148, 92, 70, 55, 44, 36, 31};
+    return std::max(1, kFit[slices] * dg_get_num_sms() / 148);
 }
 
 // CTAs along K (a cluster) for a launch with `items` blocks of 128 columns: the number with the fewest K-blocks in a row (~0.25 us each, an
 // SM's two CTAs side by side), a little more with partners, which finish an item before they begin the next
-int choose_slices(int64_t items, int num_blocks, int ctas_per_sm) {
+int choose_slices(int64_t items, int num_blocks) {
     int best = 1;
     double best_cost = 0.0;
     for (int s = 1; s <= few::kMaxCluster && (s == 1 || num_blocks / s >= 2); ++s) {
-        const double waves = static_cast<double>(ceil_div<int64_t>(items, clusters_at_once(s, ctas_per_sm)));
+        const double waves = static_cast<double>(ceil_div<int64_t>(items, clusters_at_once(s)));
         const double cost = waves * (0.25 * ceil_div(num_blocks, s) + (s > 1 ? 1.5 : 0.0));
         if (s == 1 || cost < best_cost) {
             best = s;
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* __
     // (in this order: what the product's kernel reads before it waits for this one, the weights, is then complete as well)
     griddep_wait();
     griddep_launch_dependents();
-    const int row0 = blockIdx.y * kSplitRows, r = threadIdx.x / 16, chunk = threadIdx.x % 16, row = row0 + r;
+    const int row0 = blockIdx.x * kSplitRows, r = threadIdx.x / 16, chunk = threadIdx.x % 16, row = row0 + r;
     if (threadIdx.x < kSplitRows) {
         const int mine = row0 + threadIdx.x;
         int slot = mine < m ? mine : -1;
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* __
     uint4 raw[kSplitCols / 128];
     #pragma unroll
     for (int b = 0; b < kSplitCols / 128; ++b) {
-        const int col = blockIdx.x * kSplitCols + b * 128 + chunk * 8;
+        const int col = blockIdx.y * kSplitCols + b * 128 + chunk * 8;
         raw[b] = make_uint4(0, 0, 0, 0);
         if (slot >= 0 && col < k) raw[b] = __ldg(reinterpret_cast<const uint4*>(a + row * lda + col));
     }
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* __
     split_bf16<kSplitCols / 128>(raw, hi, lo, code);
     #pragma unroll
     for (int b = 0; b < kSplitCols / 128; ++b) {
-        const int col = blockIdx.x * kSplitCols + b * 128 + chunk * 8;
+        const int col = blockIdx.y * kSplitCols + b * 128 + chunk * 8;
         if (slot >= 0 && col < k) {
             *reinterpret_cast<uint2*>(out.q + static_cast<int64_t>(slot) * k + col) = hi[b];
             *reinterpret_cast<uint2*>(out.q + (static_cast<int64_t>(out.slots) + slot) * k + col) = lo[b];
@@ -115,14 +115,14 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* __
     __syncthreads();
     if (threadIdx.x < 2 * (kSplitCols / 128) * kSplitRows) {
         const int i = threadIdx.x, rr = i % kSplitRows, b = i / kSplitRows % (kSplitCols / 128), plane = i / kSplitRows / (kSplitCols / 128);
-        const int kb = blockIdx.x * (kSplitCols / 128) + b;
+        const int kb = blockIdx.y * (kSplitCols / 128) + b;
         if (slot_of[rr] >= 0 && kb < k / 128)
             out.sf[(static_cast<int64_t>(kb) * 2 + plane) * out.slots + slot_of[rr]] = words[plane][b][rr];
     }
 }
 
 int split_rows(const dg_gemm_args_t* g, const int* group_ends, const Planes& planes) {
-    const dim3 grid(ceil_div(g->k, kSplitCols), ceil_div(g->m, kSplitRows));
+    const dim3 grid(ceil_div(g->m, kSplitRows), ceil_div(g->k, kSplitCols));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(256);
@@ -142,7 +142,7 @@ int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Plane
     // Items: exact for a dense product; a ragged one has at most one group per row, and a pass more per kTokens rows
     const int64_t tiles_n = ceil_div(g->n, 128), passes = ceil_div(g->m, kTokens);
     const int64_t items = tiles_n * (p.group_ends != nullptr ? std::min(g->m, g->num_groups + g->m / kTokens) : passes);
-    const int slices = choose_slices(items, g->k / 128, S::kCtasPerSm);
+    const int slices = choose_slices(items, g->k / 128);
     CUtensorMap tm_w, tm_sf, tm_a, tm_sfa;
     int rc;
     const uint64_t words = ceil_div(g->k, 4 * g->gran_k_b);
@@ -164,7 +164,7 @@ int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Plane
     const int smem = S::smem_bytes(slices);
     DG_CUDA_RT(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items, clusters_at_once(slices, S::kCtasPerSm))) * slices);
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items, clusters_at_once(slices))) * slices);
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(g->stream);
@@ -199,7 +199,8 @@ int launch_many_rows(const dg_gemm_args_t* g, bool ragged, const Planes& planes)
 }
 
 // Which kernels a product takes, by the rows of A that meet one matrix of weights (ragged: on average; the sizes are on the device):
-//   up to 8      the few-row kernel, splitting A itself
+//   up to 8      the few-row kernel, splitting A itself; with more weights than below, and groups that hold more than 8 rows as often as not,
+//                16 rows a pass on A split ahead (131 rows in 32 groups, N 7168 K 2048: 40 us against 49)
 //   up to 16     the same with 16 rows a pass, as long as an SM has no more than ~16 blocks of 128 x 128 weights to go through; with more of them
 //                splitting A for each costs more than a kernel that splits it once (N 7168 K 16384: 26 us against 21; N 4096 K 7168: 10.5 against 11.4)
 //   up to 32     the few-row kernel on A split ahead
@@ -207,11 +208,10 @@ int launch_many_rows(const dg_gemm_args_t* g, bool ragged, const Planes& planes)
 enum class Form { kSplit8, kSplit16, kPlanes16, kPlanes32, kMany };
 Form form_of(const dg_gemm_args_t* g, bool ragged) {
     const int rows = ragged ? ceil_div(g->m, g->num_groups) : g->m;
-    if (rows <= 8) return Form::kSplit8;
-    if (rows <= 16) {
-        const int64_t blocks = static_cast<int64_t>(ceil_div(g->n, 128)) * ceil_div(g->k, 128) * (ragged ? std::min(g->num_groups, g->m) : 1);
-        return blocks <= static_cast<int64_t>(16) * dg_get_num_sms() ? Form::kSplit16 : Form::kPlanes16;
-    }
+    const int64_t blocks = static_cast<int64_t>(ceil_div(g->n, 128)) * ceil_div(g->k, 128) * (ragged ? std::min(g->num_groups, g->m) : 1);
+    const bool many_blocks = blocks > static_cast<int64_t>(16) * dg_get_num_sms();
+    if (rows <= 8 && !(ragged && rows > 4 && many_blocks)) return Form::kSplit8;
+    if (rows <= 16) return many_blocks ? Form::kPlanes16 : Form::kSplit16;
     // (the GEMM kernel stores whole 16-byte pieces of a row of D: where N ends inside one, what follows the row would not stay)
     const int d_elem = g->d_dtype == DG_FP32 ? 4 : 2;
     return rows <= 32 || (static_cast<int64_t>(g->n) * d_elem) % 16 != 0 ? Form::kPlanes32 : Form::kMany;
@@ -236,6 +236,7 @@ int run(const dg_gemm_args_t* g, bool ragged, void* workspace, int64_t given_byt
     DG_REQUIRE(g->m >= 0 && g->n >= 0 && g->k >= 0);
     if (ragged) DG_REQUIRE(g->n > 0 && g->k > 0 && g->num_groups > 0 && g->num_groups <= 65535 && !g->accumulate && !g->has_alpha);
     else DG_REQUIRE(g->num_groups == 1);
+    DG_REQUIRE(static_cast<int64_t>(g->num_groups) * g->n <= INT32_MAX);       // rows of W as a copy's coordinate
     if (g->m == 0 || g->n == 0) return DG_OK;
     if (g->k == 0) return fail(DG_ERR_INVALID_ARGUMENT, "k == 0 must be handled by the caller (zero or copy D)");
     DG_REQUIRE(g->k % 128 == 0);                                           // as for every packed FP4 operand

@@ -813,6 +813,7 @@ int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratc
     const uint64_t bs_sfa = batched ? a->sfa_pitch * 4 * ceil_div(p.k, p.gran_k_a * 4) : 0;
     const uint64_t bs_sfb = batched ? a->sfb_pitch * 4 * ceil_div(p.k, p.gran_k_b * 4) : 0;
     CUtensorMap tm_a, tm_b, tm_sfa, tm_sfb, tm_d, tm_d_full;
+    const bool half_boxes = p.planes == 2 && cfg.cluster_size == 1;      // split A: the kernel's boxes of A and its scales are 64 rows high
     // K-major A, B: K (elements) x rows; box = one K-block (at most 128 bytes of it) x the tile's rows, swizzled over its width.
     const CUtensorMapSwizzle k_major_swizzle = cfg.block_k >= 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
     // MN-major (FP8 only): MN x (groups x K); box = 128 columns of MN x one K-block.
@@ -828,7 +829,7 @@ int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratc
         // packed operands as plain byte matrices [rows, K / 2]: a 128-byte box row is 256 elements of K
         if ((rc = encode_2d(&tm_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a->a, p.k / 2, a_rows, a->lda, 128, lay.a_stage_rows(), CU_TENSOR_MAP_SWIZZLE_128B)) != DG_OK) return rc;
     } else if (!p.a_mn_major) {
-        if ((rc = encode_2d(&tm_a, a_type, a->a, k_inner, a_rows, a->lda * ab_elem, box_k, lay.a_stage_rows(), k_major_swizzle,
+        if ((rc = encode_2d(&tm_a, a_type, a->a, k_inner, a_rows, a->lda * ab_elem, box_k, half_boxes ? 64 : lay.a_stage_rows(), k_major_swizzle,
                             nb_ab, bs_a * ab_elem)) != DG_OK) return rc;
     } else {
         if ((rc = encode_2d(&tm_a, a_type, a->a, p.m, p.k, a->lda * ab_elem, atom_mn, box_k, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -850,7 +851,7 @@ int run_gemm(int kind, const dg_gemm_args_t* a, const FixedScratch* fixed_scratc
     } else {
         // (one packed word per row and K-block, two for the 256-element stages of kind::mxf4)
         // (split A: two rows per K-block, one for each plane, in one box)
-        if ((rc = encode_2d(&tm_sfa, CU_TENSOR_MAP_DATA_TYPE_INT32, a->sfa, plane_rows > 0 ? plane_rows : p.m, sfa_rows * p.planes, a->sfa_pitch * 4, cfg.block_m,
+        if ((rc = encode_2d(&tm_sfa, CU_TENSOR_MAP_DATA_TYPE_INT32, a->sfa, plane_rows > 0 ? plane_rows : p.m, sfa_rows * p.planes, a->sfa_pitch * 4, half_boxes ? 64 : cfg.block_m,
                             lay.sfa_words() * p.planes, CU_TENSOR_MAP_SWIZZLE_NONE, nb, bs_sfa)) != DG_OK) return rc;
         if ((rc = encode_2d(&tm_sfb, CU_TENSOR_MAP_DATA_TYPE_INT32, a->sfb, p.n, sfb_rows, a->sfb_pitch * 4, lay.sf_block_n(), lay.sfb_words(),
                             CU_TENSOR_MAP_SWIZZLE_NONE, nb, bs_sfb)) != DG_OK) return rc;
@@ -976,11 +977,30 @@ int dg_m_grouped_fp8_fp4_gemm_masked(const dg_gemm_args_t* args) { return run_ge
 int dg_k_grouped_fp8_gemm_contiguous(const dg_gemm_args_t* args) { return run_gemm(DG_GEMM_K_GROUPED_CONTIGUOUS, args); }
 int dg_fp8_bmm(const dg_gemm_args_t* args) { return run_gemm(DG_GEMM_BATCHED, args); }
 
+// The problem of a shape without its pointers.  BF16 A and packed FP4 B: the many-row form of the BF16 x FP4 products, a GEMM of A's two planes
+static int describe_shape(int kind, const dg_gemm_args_t* args, Problem* p) {
+    const bool split_a = args != nullptr && args->a_dtype == DG_BF16 && args->b_dtype == DG_FP4_E2M1_X2;
+    dg_gemm_args_t planes;
+    if (split_a) {
+        planes = *args;
+        planes.a_dtype = DG_FP8_E4M3;
+        planes.gran_k_a = 32;
+        planes.lda = args->k;
+        planes.sfa_pitch = align_up(args->m, 4);
+        args = &planes;
+    }
+    DG_REQUIRE((kind == DG_GEMM_M_GROUPED_RAGGED) <= split_a);
+    DG_REQUIRE(!split_a || kind == DG_GEMM_DENSE || kind == DG_GEMM_M_GROUPED_RAGGED);
+    const int rc = validate(kind, args, false, p);
+    if (rc == DG_OK && split_a) p->planes = 2;
+    return rc;
+}
+
 int dg_get_gemm_config(int kind, const dg_gemm_args_t* args, dg_gemm_config_t* config) {
     DG_REQUIRE(config != nullptr);
     env_refresh();
     Problem p;
-    const int rc = validate(kind, args, false, &p);
+    const int rc = describe_shape(kind, args, &p);
     if (rc != DG_OK) return rc;
     DG_REQUIRE(p.m > 0 && p.n > 0 && p.k > 0);
     return choose_config(p, config);
@@ -989,7 +1009,7 @@ int dg_get_gemm_config(int kind, const dg_gemm_args_t* args, dg_gemm_config_t* c
 int dg_gemm_precompile(int kind, const dg_gemm_args_t* args) {
     env_refresh();
     Problem p;
-    int rc = validate(kind, args, false, &p);
+    int rc = describe_shape(kind, args, &p);
     if (rc != DG_OK) return rc;
     DG_REQUIRE(p.m > 0 && p.n > 0 && p.k > 0);
     dg_gemm_config_t cfg;

@@ -229,8 +229,8 @@ DG_API int dg_fp8_bmm(const dg_gemm_args_t* args);
  * groups and no alignment; ends must not decrease; rows at or behind the last end are not written.
  * Sums are FP32, one rounding per element of D.  A row of A with an infinity or a NaN gives non-finite results.
  * workspace: device memory of this call alone until it has completed, 128-byte aligned, at least
- * dg_bf16_fp4_workspace_bytes(args, ragged) bytes (0 up to eight rows per matrix of weights; about 2 m k above; reads only the
- * sizes in args; -1: no valid sizes). */
+ * dg_bf16_fp4_workspace_bytes(args, ragged) bytes (0 for a few rows per matrix of weights, about 2 m k above; it reads only the
+ * sizes, num_groups and d_dtype in args; -1: no valid sizes). */
 DG_API int64_t dg_bf16_fp4_workspace_bytes(const dg_gemm_args_t* args, int ragged);
 DG_API int dg_bf16_fp4_gemm(const dg_gemm_args_t* args, void* workspace_device, int64_t workspace_bytes);
 DG_API int dg_m_grouped_bf16_fp4_gemm_ragged(const dg_gemm_args_t* args, void* workspace_device, int64_t workspace_bytes);
@@ -253,7 +253,9 @@ DG_API int dg_m_grouped_bf16_fp4_gemm_ragged(const dg_gemm_args_t* args, void* w
 DG_API int dg_fp8_fp4_gemm_noalloc(const dg_gemm_args_t* args);
 
 /* Compile (but do not load or launch) the kernel the call above would use, so that a later call
- * finds it in the cache.  Needs nvcc, not a GPU.  Device pointers in `args` may be null. */
+ * finds it in the cache.  Needs nvcc, not a GPU.  Device pointers in `args` may be null.  a_dtype DG_BF16 with b_dtype
+ * DG_FP4_E2M1_X2 (kind DG_GEMM_DENSE or DG_GEMM_M_GROUPED_RAGGED; here and in dg_get_gemm_config): the GEMM that
+ * dg_bf16_fp4_gemm / dg_m_grouped_bf16_fp4_gemm_ragged run for many rows. */
 DG_API int dg_gemm_precompile(int kind, const dg_gemm_args_t* args);
 
 /* ---- heuristics: csrc/jit_kernels/heuristics/{common,sm100}.hpp -------------------------------- */

@@ -67,3 +67,38 @@ def test_workspace():
     for kw in (dict(workspace=None), dict(workspace=0x7000, given=100), dict(workspace=0x7040), dict(workspace=0x7000, given=-1)):
         assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(m=64)), kw.get("workspace"), kw.get("given", 1 << 20)) != _lib.DG_OK
         assert "workspace" in _lib.last_error()
+
+
+@pytest.mark.parametrize("counts", [[0, 0, 5], [1] * 8, [130, 0, 1, 63, 257], [64, 65, 128, 129, 0], [0, 0, 0], [1000]])
+@pytest.mark.parametrize("ctas", [1, 7, 148])
+def test_the_ragged_scheduler_visits_every_tile_of_every_group_once(counts, ctas):
+    """The many-row form's walk: (first row of the tile in D, column block, group, rows that count), shared by all CTAs."""
+    n, block_n = 500, 96
+    ends = (C.c_int32 * len(counts))(*[sum(counts[:i + 1]) for i in range(len(counts))])
+    seen = []
+    for cta in range(ctas):
+        out = (C.c_uint32 * 4096)()
+        got = _lib.lib.dg_enumerate_tiles(_lib.DG_GEMM_M_GROUPED_RAGGED, block_n, 4, max(1, sum(counts)), n, len(counts), ends, cta, ctas, out, 1024)
+        seen += [tuple(out[4 * i:4 * i + 4]) for i in range(got)]
+    want = []
+    for g, c in enumerate(counts):
+        first = sum(counts[:g])
+        for b in range(-(-c // 128)):
+            want += [(first + 128 * b, j, g, min(128, c - 128 * b)) for j in range(-(-n // block_n))]
+    assert sorted(seen) == sorted(want)
+
+
+def test_the_many_row_configurations():
+    """A stage holds 128 rows of both planes; CTA pairs for large dense products only; K slices only inside a cluster."""
+    for m in (40, 64, 129, 300, 1024, 4096):
+        for n, k in ((2112, 7168), (24576, 1536), (256, 128), (7168, 16384)):
+            for kind, groups in ((_lib.DG_GEMM_DENSE, 1), (_lib.DG_GEMM_M_GROUPED_RAGGED, 8)):
+                cfg = dg.get_gemm_config(kind, m, n, k, num_groups=groups, a_is_bf16=True, b_is_fp4=True, gran_k_b=32)
+                assert cfg["block_m"] == 128 and cfg["block_k"] == 128 and cfg["num_stages"] >= 2 and not cfg["swap_ab"]
+                assert cfg["smem_bytes"] <= 232448 and cfg["tmem_cols"] <= 512
+                assert cfg["num_splits"] == 1 or cfg["split_in_cluster"]
+                assert cfg["cluster_size"] == 1 or (kind == _lib.DG_GEMM_DENSE and m >= 1024)
+    with pytest.raises(RuntimeError):
+        dg.get_gemm_config(_lib.DG_GEMM_M_GROUPED_RAGGED, 256, 512, 512, num_groups=2, b_is_fp4=True, gran_k_b=32)
+    with pytest.raises(RuntimeError):
+        dg.get_gemm_config(_lib.DG_GEMM_M_GROUPED_MASKED, 256, 512, 512, num_groups=2, expected_m=8, a_is_bf16=True, b_is_fp4=True, gran_k_b=32)

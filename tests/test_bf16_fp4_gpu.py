@@ -83,7 +83,7 @@ def check_product(d, a, w, added=None, alpha=1.0):
 
 DENSE = [(1, 8, 128), (1, 2112, 7168), (1, 264, 16384), (2, 24, 256), (5, 100, 384), (7, 1544, 1536), (8, 40, 1152), (9, 136, 640), (15, 72, 896),
          (16, 4096, 512), (17, 48, 2048), (31, 256, 1024), (32, 80, 128), (33, 264, 2048), (61, 520, 384), (64, 576, 1152), (65, 512, 256),
-         (127, 128, 3200), (128, 2112, 512), (129, 256, 512), (300, 1000, 768), (511, 136, 128), (1030, 520, 384), (2500, 1032, 1280)]
+         (40, 96, 256), (127, 128, 3200), (192, 1544, 256), (193, 264, 1024), (128, 2112, 512), (129, 256, 512), (300, 1000, 768), (511, 136, 128), (1030, 520, 384), (2500, 1032, 1280)]
 
 
 @pytest.mark.parametrize("m,n,k", DENSE)
@@ -100,7 +100,7 @@ def test_dense(m, n, k, gran, out):
     assert dg.kernel_status() == 0
 
 
-@pytest.mark.parametrize("m", [1, 6, 40, 200, 600])
+@pytest.mark.parametrize("m", [1, 6, 14, 40, 64, 150, 200, 600])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float])
 @pytest.mark.parametrize("in_place", [True, False])
 def test_dense_accumulates_and_scales(m, out, in_place):
@@ -171,7 +171,7 @@ def test_fp32_scales_give_the_bits_of_packed_ones():
 
 
 RAGGED = [([1], 0), ([0, 0, 5], 2), ([1] * 8, 0), ([3, 0, 11, 0, 0, 2, 1], 4), ([0, 17, 33, 8, 0, 64, 65, 1], 0), ([130, 0, 1, 63, 257], 7),
-          ([0, 0, 0], 6), ([128, 256, 384], 0), ([500, 1, 2, 499], 1), ([1, 2, 3, 4] * 20, 3), ([40] * 24, 0), ([901], 0), ([0, 700, 0, 13], 5)]
+          ([64, 65, 128, 129, 192, 193, 1, 0, 63], 2), ([320, 64, 200, 0, 1], 0), ([0, 0, 0], 6), ([128, 256, 384], 0), ([500, 1, 2, 499], 1), ([1, 2, 3, 4] * 20, 3), ([40] * 24, 0), ([901], 0), ([0, 700, 0, 13], 5)]
 
 
 def ragged_case(counts, spare, n, k, gran, seed):
