@@ -33,7 +33,8 @@ struct GemmLayout {
                                                    // memory and lands in accumulator rows that are never stored
 
     uint32_t planes = 1;                           // 2: A is a BF16 matrix split into two E4M3 planes; a stage holds block_m rows of each, both
-                                                   // multiplied with the stage's B into one accumulator
+                                                   // multiplied with the stage's B into one accumulator (a_rows == 64: 64 rows of each, one above
+                                                   // the other in one MMA)
 
     // A packed scale word covers 4 * gran_k elements of K: it is fetched on every `period`-th K-block of a work item,
     // into the next of a ring of buffers.  A buffer may be refilled once the fetch it held is no longer among the
@@ -79,7 +80,7 @@ struct GemmLayout {
     // MN-major only: atoms of [block_k / ab_elem_bytes rows of K][128 bytes of N]
     DG_HDC uint32_t b_atoms() const { return (load_block_n() * ab_elem_bytes + 127) / 128; }
     DG_HDC uint32_t b_bytes() const { return b_mn_major ? b_atoms() * 128 * (block_k / ab_elem_bytes) : load_block_n() * block_k; }
-    DG_HDC uint32_t sfa_bytes() const { return block_m * 4 * sfa_words() * planes; }          // [word of K][row] int32 ([plane][row] with two planes)
+    DG_HDC uint32_t sfa_bytes() const { return (planes == 2 ? a_stage_rows() : block_m) * 4 * sfa_words() * planes; }          // [word of K][row] int32 ([plane][row] with two planes)
     DG_HDC uint32_t sfb_bytes() const { return sf_block_n() * 4 * sfb_words(); }
 
     DG_HDC uint32_t off_d() const { return 0; }

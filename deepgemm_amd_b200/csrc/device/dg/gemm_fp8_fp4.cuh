@@ -150,11 +150,15 @@ constexpr uint32_t kL2Hint     = DG_L2_HINT;
 #endif
 constexpr uint32_t kPlanes     = DG_PLANES;        // E4M3 matrices that make up A
 constexpr bool     kHalfTiles  = kPlanes == 2 && kCluster == 1;
+#ifndef DG_A_ROWS
+#define DG_A_ROWS 0
+#endif
+constexpr bool     kAllHalf    = kHalfTiles && DG_A_ROWS == 64;      // every tile has at most 64 rows, and the stages hold no more
 
 constexpr uint32_t UMMA_M = 128 * kCluster, UMMA_N = BLOCK_N, UMMA_K = 32;
 constexpr uint32_t LOAD_BLOCK_N = BLOCK_N / kCluster;      // rows of B each CTA loads
 constexpr uint32_t CTA_M = BLOCK_M * kMHalves;             // rows of A (and D) per CTA
-constexpr uint32_t TILE_M = CTA_M * kCluster;              // rows of D per scheduled tile
+constexpr uint32_t TILE_M = kAllHalf ? 64 : CTA_M * kCluster;        // rows of D per scheduled tile
 // Four role warps and one epilogue warpgroup per 128 rows of the CTA's tile
 constexpr uint32_t kNumThreads = 128 + 128 * kMHalves, kNumEpilogueThreads = 128, kEpilogueWarpBase = 4;
 // Tensor memory holds two accumulators: two tiles in flight, or the two halves of one
@@ -232,15 +236,12 @@ static_assert(kSplitCluster == 1 || (kGemmType == kDense && !kSplitK && kCluster
 #ifndef DG_EPILOGUE_BACKOFF_NS
 #define DG_EPILOGUE_BACKOFF_NS 0
 #endif
-#ifndef DG_A_ROWS
-#define DG_A_ROWS 0
-#endif
 constexpr GemmLayout kLayout{CTA_M, BLOCK_N, BLOCK_K, kNumStages, kDElemBytes, kCluster, kBMnMajor ? 1u : 0u, kGranKA, kGranKB,
                              DG_SHORT_K, kABElemBytes, DG_STORE_BUFFERS, kMXF4 ? 1u : 0u, DG_A_ROWS, kPlanes};
-static_assert(DG_A_ROWS == 0 || (DG_A_ROWS % 8 == 0 && DG_A_ROWS < 128 && kGemmType == kDense && kCluster == 1 && kMHalves == 1 && !kAMnMajor),
-              "a shortened A stage: dense GEMMs with fewer rows than one tile, K-major A, one CTA per tile");
+static_assert(DG_A_ROWS == 0 || (DG_A_ROWS % 8 == 0 && DG_A_ROWS < 128 && (kGemmType == kDense || kAllHalf) && kCluster == 1 && kMHalves == 1 && !kAMnMajor),
+              "a shortened A stage: dense GEMMs with fewer rows than one tile (or a split A in tiles of 64), K-major A, one CTA per tile");
 static_assert(kPlanes == 1 || (kPlanes == 2 && kMHalves == 1 && kHasSF && !kMXF4 && !kAIsFP4 && !kAMnMajor && !kBMnMajor && BLOCK_K == 128 && kGranKA == 32 &&
-                               DG_A_ROWS == 0 && !kTransposedD && (kGemmType == kDense || kGemmType == kMGroupedRagged)),
+                               (DG_A_ROWS == 0 || kAllHalf) && !kTransposedD && (kGemmType == kDense || kGemmType == kMGroupedRagged)),
               "split A: K-major E4M3 planes with one scale per 32 elements, 128 rows per CTA, dense and ragged");
 static_assert(kGemmType != kMGroupedRagged || (kPlanes == 2 && kCluster == 1), "ragged groups: built for a split A, one CTA per tile");
 constexpr uint32_t kSFAWords = kHasSF ? kLayout.sfa_words() : 1, kSFBWords = kHasSF ? kLayout.sfb_words() : 1;   // packed words per row and stage
@@ -474,6 +475,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
     // Split A: whether the tile has at most 64 rows that count
     auto is_half = [&](const Tile& t) {
         if constexpr (!kHalfTiles) return false;
+        if constexpr (kAllHalf) return true;
         return (kGemmType == kDense ? p.shape_m - t.m_block * TILE_M : t.valid_rows) <= 64;
     };
     // Every role walks the same sequence of (pass, K-block) steps of a tile, one pipeline stage per step
@@ -551,7 +553,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                         [[maybe_unused]] const bool half = is_half(tile);
                         if constexpr (kHasSF) {
                             uint32_t sf_bytes = 0;
-                            if (kb % kSFAPeriod == 0) sf_bytes += half ? kSFABytes / 2 : kSFABytes;
+                            if (kb % kSFAPeriod == 0) sf_bytes += half && !kAllHalf ? kSFABytes / 2 : kSFABytes;
                             if (kb % kSFBPeriod == 0) sf_bytes += kSFBBytes;
                             mbar_arrive_expect_tx(sf_full_bar(stage), sf_bytes);
                             if (kb % kSFAPeriod == 0)
@@ -565,7 +567,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                         // With a cluster the copies land in this CTA and their bytes are counted on CTA 0's barrier,
                         // which expects both CTAs' bytes
                         const uint32_t load_bar = kCluster == 1 ? full_bar(stage) : in_leader(full_bar(stage));
-                        if (kCluster == 1 || is_leader) mbar_arrive_expect_tx(full_bar(stage), kTxBytesAB - (half ? kABytes / 2 : 0u));
+                        if (kCluster == 1 || is_leader) mbar_arrive_expect_tx(full_bar(stage), kTxBytesAB - (half && !kAllHalf ? kABytes / 2 : 0u));
                         else mbar_arrive_cluster(load_bar);
                         auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y) {
                             if constexpr (kL2Hint != 0 && kGemmType != kBatched) {

@@ -203,8 +203,9 @@ int launch_many_rows(const dg_gemm_args_t* g, bool ragged, const Planes& planes)
 //                16 rows a pass on A split ahead (131 rows in 32 groups, N 7168 K 2048: 40 us against 49)
 //   up to 16     the same with 16 rows a pass, as long as an SM has no more than ~16 blocks of 128 x 128 weights to go through; with more of them
 //                splitting A for each costs more than a kernel that splits it once (N 7168 K 16384: 26 us against 21; N 4096 K 7168: 10.5 against 11.4)
-//   up to 32     the few-row kernel on A split ahead
-//   above        the GEMM kernel on A split ahead (N 7168 K 2048: 11.4 us at 64 rows, the few-row kernel 13.3)
+//   up to 32     the few-row kernel on A split ahead, 32 rows a pass (ragged: up to 24, a pass that a group's size leaves half empty costs
+//                as much as a full one: 320 rows in 16 groups, N 4096 K 7168: 63 us against 70 below, 400 rows 80 against 78)
+//   above        the GEMM kernel on A split ahead (48 rows, N 4096 K 7168: 13.5 us, the few-row kernel in two passes 14.6; 32 rows: 12.8 against 11.4)
 enum class Form { kSplit8, kSplit16, kPlanes16, kPlanes32, kMany };
 Form form_of(const dg_gemm_args_t* g, bool ragged) {
     const int rows = ragged ? ceil_div(g->m, g->num_groups) : g->m;
@@ -214,7 +215,7 @@ Form form_of(const dg_gemm_args_t* g, bool ragged) {
     if (rows <= 16) return many_blocks ? Form::kPlanes16 : Form::kSplit16;
     // (the GEMM kernel stores whole 16-byte pieces of a row of D: where N ends inside one, what follows the row would not stay)
     const int d_elem = g->d_dtype == DG_FP32 ? 4 : 2;
-    return rows <= 32 || (static_cast<int64_t>(g->n) * d_elem) % 16 != 0 ? Form::kPlanes32 : Form::kMany;
+    return rows <= (ragged ? 24 : 32) || (static_cast<int64_t>(g->n) * d_elem) % 16 != 0 ? Form::kPlanes32 : Form::kMany;
 }
 bool splits_inside(const dg_gemm_args_t* g, bool ragged) {
     const Form form = form_of(g, ragged);

@@ -340,13 +340,19 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
         // K-major FP8 operands with one scale per 128 elements, 128-row CTAs, K a whole number of such stages
         if (bk == 256 && (p.kind != DG_GEMM_DENSE || p.a_fp4 || p.b_fp4 || p.ab_bf16 || p.mxf4 || p.a_mn_major || p.b_mn_major || p.gran_k_a != 128 ||
                           p.gran_k_b != 128 || p.reduce_batches > 1 || cluster != 1 || halves != 1 || p.k % 256 != 0)) continue;
-        const int tile_m = 128 * cluster * halves, units = num_sms / cluster;
+        const int units = num_sms / cluster;
         // A dense GEMM with at most 64 rows stages only those rows of A (16, 32 or 64; the box of its tensor map): the
         // bytes saved per stage become more stages, i.e. more of B in flight.  DG_FORCE_A_ROWS=128 keeps whole tiles.
         int a_rows = 0;
         if (p.kind == DG_GEMM_DENSE && cluster == 1 && halves == 1 && bk >= 128 && !p.a_mn_major && p.reduce_batches <= 1 && p.m <= 64 && p.planes == 1 &&
             env_int("FORCE_A_ROWS") != 128)
             a_rows = p.m <= 16 ? 16 : (p.m <= 32 ? 32 : 64);
+        // A split A: tiles of 64 rows, both planes in one MMA, where the rows of a matrix of weights are few: the stages, half as high, become more
+        // (61 rows, N 7168 K 2048: 10.2 -> 9.6 us; 64 rows, N 4096 K 7168: 16.7 -> 13.6).  Ragged, by the average group, measured over
+        // 16 groups of N 4096 K 7168: 120 us against 127 at 94 rows, 163 against 152 at 125
+        if (p.planes == 2 && cluster == 1 && env_int("FORCE_A_ROWS") != 128 && (p.kind == DG_GEMM_DENSE ? p.m <= 64 : p.m <= static_cast<int64_t>(96) * p.groups))
+            a_rows = 64;
+        const int tile_m = p.planes == 2 && a_rows ? a_rows : 128 * cluster * halves;
         int64_t m_blocks;
         if (p.kind == DG_GEMM_M_GROUPED_MASKED)
             m_blocks = static_cast<int64_t>(p.groups) * ceil_div(std::min(std::max(p.expected_m, 1), p.m), tile_m);
@@ -401,10 +407,12 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
                 const int64_t item_kb = ceil_div<int64_t>(item_k, bk);
                 int max_stages = static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(32, 2 * item_kb)));
                 if (forced_stages >= 2) max_stages = std::min(max_stages, forced_stages);
+                // (tiles of 64 rows: one staging buffer, a ragged tile stores row by row anyway)
+                const uint32_t store_buffers = p.planes == 2 && a_rows ? 1u : 2u;
                 GemmLayout lay{128u * halves, static_cast<uint32_t>(bn), static_cast<uint32_t>(bk), 2,
                                static_cast<uint32_t>(splits > 1 && !in_cluster ? 4 : d_elem), static_cast<uint32_t>(cluster),
                                p.b_mn_major ? 1u : 0u, static_cast<uint32_t>(p.gran_k_a), static_cast<uint32_t>(p.gran_k_b), 0u,
-                               static_cast<uint32_t>(ab_elem), 2u, p.mxf4 ? 1u : 0u, static_cast<uint32_t>(a_rows), static_cast<uint32_t>(p.planes)};
+                               static_cast<uint32_t>(ab_elem), store_buffers, p.mxf4 ? 1u : 0u, static_cast<uint32_t>(a_rows), static_cast<uint32_t>(p.planes)};
                 const GemmLayout unfitted = lay;
                 lay = fit_stages(lay, p.kind == DG_GEMM_K_GROUPED_CONTIGUOUS ? 0 : item_kb, max_stages);   // slices may be one K-block
                 if (lay.num_stages <= 2 && env_int("FORCE_STORE_BUFFERS") != 2) {
@@ -418,7 +426,7 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
                 // The cost model was fitted on whole-tile A stages: a shortened A stage keeps the model's choice of tile
                 // and slicing and only deepens that candidate's pipeline
                 uint32_t model_stages = lay.num_stages;
-                if (a_rows) {
+                if (a_rows && p.planes == 1) {
                     GemmLayout whole = unfitted;
                     whole.a_rows = 0;
                     whole.store_buffers = lay.store_buffers;
@@ -435,7 +443,7 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
                 // and its B rows once per 128-row half), and into which no configuration pulled more than ~67 B per cycle
                 // from L2; and the ring of stages, `stages` of which complete per (load latency + MMA time).
                 const double stage_frac = bk / 128.0;
-                const int a_parts = halves * p.planes;          // 128-row pieces of A per stage, each multiplied with the stage's B
+                const int a_parts = a_rows ? 1 : halves * p.planes;      // 128-row pieces of A per stage, each multiplied with the stage's B
                 const double mma = 2.0 * bn * a_parts * stage_frac;
                 const double stage_bytes = (128.0 * a_parts + static_cast<double>(bn) / cluster) * bk;
                 // (with a CTA pair the peer's tensor core reads this CTA's half of B as well)

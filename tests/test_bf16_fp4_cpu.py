@@ -97,6 +97,7 @@ def test_the_many_row_configurations():
                 assert cfg["block_m"] == 128 and cfg["block_k"] == 128 and cfg["num_stages"] >= 2 and not cfg["swap_ab"]
                 assert cfg["smem_bytes"] <= 232448 and cfg["tmem_cols"] <= 512
                 assert cfg["num_splits"] == 1 or cfg["split_in_cluster"]
+                assert cfg["a_rows"] == (64 if m <= 64 or (groups > 1 and m <= 96 * groups) else 128)
                 assert cfg["cluster_size"] == 1 or (kind == _lib.DG_GEMM_DENSE and m >= 1024)
     with pytest.raises(RuntimeError):
         dg.get_gemm_config(_lib.DG_GEMM_M_GROUPED_RAGGED, 256, 512, 512, num_groups=2, b_is_fp4=True, gran_k_b=32)

@@ -7,7 +7,7 @@ Tolerance.  Per element, with S = sum |a| |w| over K:
   * a product of a BF16 value, an E2M1 value and a power of two is exact; the sums are chains of at most K / 8 + 64
     FP32 additions (eight or more products meet in one tensor-core or FMA step), each off by at most 2^-23 of a partial
     sum that S bounds: (K / 8 + 64) 2^-23 S;
-  * many rows of A are split into two E4M3 values per element with one scale per 32 elements of K: what the split cannot hold is
+  * rows of A are split into two E4M3 values per element with one scale per 32 elements of K: what the split cannot hold is
     below 2^-14 of that scale, and the scale is at most 2^-7 of the block's largest element (amax / 448 rounded up to a power
     of two is below amax / 224): 2^-21 amax |w|, summed over K;
   * scaling by alpha: one more FP32 rounding, inside the slack of the second term.
@@ -277,6 +277,138 @@ def test_two_streams_and_two_graphs_at_once(m):
     torch.cuda.synchronize()
     for s in sides:
         check_product(s["d"], s["a"], s["w"])
+
+
+FORMS = [1, 8, 14, 24, 48, 200]                    # rows of A: one count for each way a dense product is computed
+RAGGED_FORMS = [3, 7, 12, 20, 40, 150]             # ... rows of an average group
+
+
+@pytest.mark.parametrize("average", RAGGED_FORMS)
+@pytest.mark.parametrize("groups", [33, 300])
+def test_many_groups(groups, average):
+    """More groups than a warp has lanes, sizes from zero to twice the average."""
+    n, k = 264, 640
+    counts = torch.randint(0, 2 * average + 1, (groups,), generator=torch.Generator().manual_seed(groups + average)).tolist()
+    codes, e, w, a, ends = ragged_case(counts, 2, n, k, 32, 90)
+    sf, first = pack_scales(e), None
+    for _ in range(2):
+        d = torch.full((a.size(0), n), -7.0, dtype=torch.bfloat16, device="cuda")
+        dg.m_grouped_bf16_fp4_gemm_nt_ragged(a, (codes, sf), d, ends)
+        assert first is None or torch.equal(first, d)
+        first = d
+    check_ragged(d, a, w, counts, -7.0)
+    assert dg.kernel_status() == 0
+
+
+@pytest.mark.parametrize("n,k,gran", [(4096, 2176, 128), (136, 16384, 32), (20000, 256, 32)])
+@pytest.mark.parametrize("m", FORMS)
+def test_slices_and_passes_of_every_form(m, n, k, gran):
+    """K in slices that do not divide it, more blocks of columns than run at once, column counts that end inside a block."""
+    codes, e, w = make_weights((n, k), gran, 100 + m)
+    a = make_rows(m, k, 101)
+    d = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    dg.bf16_fp4_gemm_nt(a, (codes, pack_scales(e)), d, recipe_b=(1, gran))
+    check_product(d, a, w)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("m", FORMS)
+def test_operands_written_just_before_and_read_just_after(m, captured):
+    """The kernels start before their predecessor has ended: what that one writes (weights, scales, rows) is what they read, and their results
+    are complete for what follows.  Two products in a row, the second one's A and weights made from the first one's results."""
+    n, k = 1024, 1024
+    (c0, e0, w0), (c1, e1, w1) = make_weights((n, k), 32, 110), make_weights((k, n), 32, 111)
+    sf0, sf1 = pack_scales(e0), pack_scales(e1)
+    a0, a1 = make_rows(m, k, 112), make_rows(m, k, 113)
+    a, codes, sf = a0.clone(), c0.clone(), sf0.clone()
+    mid, out, last = (torch.empty((m, n), dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    dg.bf16_fp4_gemm_nt(a, (codes, sf), mid)           # kernels loaded ahead of a capture
+
+    def run():
+        for rows, w, scales in ((a0, c0, sf0), (a1, c1, sf1)):
+            a.copy_(rows)
+            codes.copy_(w)
+            sf.copy_(scales)
+            dg.bf16_fp4_gemm_nt(a, (codes, sf), mid)
+            dg.bf16_fp4_gemm_nt(mid, (codes, sf), out)
+            last.copy_(out)
+
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+    for _ in range(10):
+        last.fill_(float("nan"))
+        graph.replay() if captured else run()
+    torch.cuda.synchronize()
+    check_product(mid, a1, w1)
+    check_product(last, mid, w1)
+
+
+@pytest.mark.parametrize("average", RAGGED_FORMS)
+def test_ends_written_just_before(average):
+    groups, n, k = 40, 520, 512
+    codes, e, w = make_weights((groups, n, k), 32, 120)
+    sf, rows = pack_scales(e), groups * average
+    a, d = make_rows(rows, k, 121), torch.empty((rows, n), dtype=torch.bfloat16, device="cuda")
+    ends = torch.zeros(groups, dtype=torch.int32, device="cuda")
+    for seed in range(4):
+        counts = torch.bincount(torch.randint(0, groups, (rows - seed,), generator=torch.Generator().manual_seed(seed)), minlength=groups)
+        ready = counts.to("cuda")
+        d.fill_(-7.0)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            ends.zero_()
+            ends.copy_(ready.cumsum(0))
+            dg.m_grouped_bf16_fp4_gemm_nt_ragged(a, (codes, sf), d, ends)
+        check_ragged(d, a, w, counts.tolist(), -7.0)
+
+
+@pytest.mark.parametrize("average", RAGGED_FORMS)
+def test_ragged_calls_in_flight_together(average):
+    groups, n, k = 12, 1024, 768
+    sides = []
+    for i in range(2):
+        counts = torch.randint(0, 2 * average + 1, (groups,), generator=torch.Generator().manual_seed(130 + i)).tolist()
+        codes, e, w, a, ends = ragged_case(counts, 1, n, k, 32, 131 + i)
+        sides.append({"args": (a, (codes, pack_scales(e)), torch.full((a.size(0), n), -7.0, dtype=torch.bfloat16, device="cuda"), ends), "w": w, "counts": counts,
+                      "stream": torch.cuda.Stream()})
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s in sides:
+            with torch.cuda.stream(s["stream"]):
+                dg.m_grouped_bf16_fp4_gemm_nt_ragged(*s["args"])
+    torch.cuda.synchronize()
+    for s in sides:
+        check_ragged(s["args"][2], s["args"][0], s["w"], s["counts"], -7.0)
+
+
+@pytest.mark.parametrize("m", FORMS)
+def test_the_compiled_binding_and_the_ctypes_one_give_the_same_bits(m, monkeypatch):
+    n, k, groups = 520, 1152, 3
+    codes, e, _ = make_weights((groups, n, k), 128, 140)
+    sf, a, c = pack_scales(e), make_rows(m, k, 141), torch.randn((m, n), device="cuda")
+    ends = torch.tensor([m // 3, m // 3, m], dtype=torch.int32, device="cuda")
+    got = []
+    for binding in (dg.api._C, None):
+        monkeypatch.setattr(dg.api, "_C", binding)
+        for dtype in (torch.bfloat16, torch.float):
+            d = torch.zeros((m, n), dtype=dtype, device="cuda")
+            dg.bf16_fp4_gemm_nt(a, (codes[1], sf[1]), d, c.to(dtype), recipe_b=(1, 128), alpha=0.375)
+            got.append(d)
+        d = torch.zeros((m, n), dtype=torch.bfloat16, device="cuda")
+        dg.m_grouped_bf16_fp4_gemm_nt_ragged(a, (codes, sf), d, ends, recipe_b=(1, 128))
+        got.append(d)
+    assert all(torch.equal(x, y) for x, y in zip(got[:3], got[3:]))
+
+
+def test_more_than_a_million_rows():
+    m, n, k = 1_100_001, 24, 128
+    codes, e, w = make_weights((n, k), 32, 150)
+    a = make_rows(m, k, 151)
+    d = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    dg.bf16_fp4_gemm_nt(a, (codes, pack_scales(e)), d)
+    check_product(d, a, w)
 
 
 def test_weights_beyond_32_bit_offsets():
