@@ -439,8 +439,12 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
     // Everything above touched no global memory, so with programmatic dependent launch it overlapped the tail of the
     // kernel before this one; from here on its results (and its reads of D) must be complete.  The kernel after
     // this one may begin its own set-up as soon as SMs free up.
-    griddep_wait();
-    griddep_launch_dependents();
+    // (Split A: what the kernel before this one wrote is A alone, and it had waited for everything before it when it let this one start, so
+    // the producer asks for the first stages of B first: 64 rows, N 4096 K 7168, 12.8 us against 13.6)
+    if (kPlanes == 1 || warp_idx != 0) {
+        griddep_wait();
+        griddep_launch_dependents();
+    }
 
     const uint32_t num_k_blocks = (p.shape_k + BLOCK_K_ELEMS - 1) / BLOCK_K_ELEMS;
     const uint32_t sfa_rows_per_group = (p.shape_k + kGranKA * 4 - 1) / (kGranKA * 4);   // packed K extent of SFA
@@ -492,6 +496,17 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
         if (kb % kSFAPeriod == 0) sfa_slot = sfa_slot + 1 == kNumSFABuffers ? 0 : sfa_slot + 1;
         if (kb % kSFBPeriod == 0) sfb_slot = sfb_slot + 1 == kNumSFBBuffers ? 0 : sfb_slot + 1;
     };
+    // The producer's announcements of a stage's copies
+    auto expect_sf = [&](uint32_t s, uint32_t kb, const Tile& t) {
+        uint32_t bytes = 0;
+        if (kb % kSFAPeriod == 0) bytes += is_half(t) && !kAllHalf ? kSFABytes / 2 : kSFABytes;
+        if (kb % kSFBPeriod == 0) bytes += kSFBBytes;
+        mbar_arrive_expect_tx(sf_full_bar(s), bytes);
+    };
+    auto expect_ab = [&](uint32_t s, const Tile& t) {
+        if (kCluster == 1 || is_leader) mbar_arrive_expect_tx(full_bar(s), kTxBytesAB - (is_half(t) && !kAllHalf ? kABytes / 2 : 0u));
+        else mbar_arrive_cluster(in_leader(full_bar(s)));
+    };
     // Tensor-map copies: two-dimensional, or with the batch as third coordinate
     auto tma_in = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, uint32_t x, uint32_t y, uint32_t batch) {
         if constexpr (kGemmType == kBatched) tma_load_3d(dst, map, bar, static_cast<int32_t>(x), static_cast<int32_t>(y), static_cast<int32_t>(batch));
@@ -529,6 +544,30 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                 [[maybe_unused]] const uint64_t policy_keep = kL2Hint ? l2_policy_evict_last() : 0, policy_stream = kL2Hint ? l2_policy_evict_first() : 0;
                 DG_PROF_VAR(prof_wait);
                 DG_PROF_BEGIN(prof_t0);
+                uint32_t ahead = 0;              // split A: steps whose barriers and copies of B and its scales are already under way
+                if constexpr (kPlanes == 2) {
+                    TileScheduler<kGemmType> peek = sched;
+                    if (peek.next(tile)) {
+                        const uint32_t kb0 = kb_begin(tile), num_kb = kb_end(tile) - kb0, b_row = tile.group * p.shape_n + tile.n_block * BLOCK_N + cta_rank * LOAD_BLOCK_N;
+                        for (; ahead < kNumStages && ahead < num_kb; ++ahead) {
+                            const uint32_t kb = kb0 + ahead;
+                            if (lane == 0) {
+                                const uint32_t load_bar = kCluster == 1 ? full_bar(ahead) : in_leader(full_bar(ahead));
+                                expect_sf(ahead, kb, tile);
+                                if (kb % kSFBPeriod == 0)
+                                    tma_in(sfb_buffer(), &tm_sfb, sf_full_bar(ahead), tile.n_block * BLOCK_N, tile.group * sfb_rows_per_group + kb / kSFBPeriod * kSFBWords, tile.group);
+                                expect_ab(ahead, tile);
+                                if constexpr (kCluster == 1) tma_load_2d(smem_base + kSmemB + ahead * kBBytes, &tm_b, load_bar, static_cast<int32_t>(kb * kLoadXPerKBlock), static_cast<int32_t>(b_row));
+                                else tma_load_2d_2cta(smem_base + kSmemB + ahead * kBBytes, &tm_b, load_bar, static_cast<int32_t>(kb * kLoadXPerKBlock), static_cast<int32_t>(b_row));
+                            }
+                            advance_sf(kb);
+                        }
+                        sfa_slot = sfb_slot = 0;
+                    }
+                    __syncwarp();
+                    griddep_wait();
+                    griddep_launch_dependents();
+                }
                 while (ok && sched.next(tile)) {
                     // Row coordinates of this CTA's part of the tile in the 2-D views of A, B and the scale tensors
                     const uint32_t a_row = tile.a_row_base + tile.m_block * TILE_M + cta_rank * CTA_M;
@@ -549,26 +588,24 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                         if (!mbar_wait(empty_bar(stage), phase ^ 1, ctx, kRoleProducer, 1)) { ok = false; break; }
                         DG_PROF_ADD(prof_wait, prof_w);
                         if constexpr (kProducerWholeWarp) __syncwarp();
+                        const bool asked = kPlanes == 2 && ahead > 0;
+                        if (asked) --ahead;
                         if (kProducerWholeWarp && lane != 0) { advance_sf(kb); continue; }
                         [[maybe_unused]] const bool half = is_half(tile);
                         if constexpr (kHasSF) {
-                            uint32_t sf_bytes = 0;
-                            if (kb % kSFAPeriod == 0) sf_bytes += half && !kAllHalf ? kSFABytes / 2 : kSFABytes;
-                            if (kb % kSFBPeriod == 0) sf_bytes += kSFBBytes;
-                            mbar_arrive_expect_tx(sf_full_bar(stage), sf_bytes);
+                            if (!asked) expect_sf(stage, kb, tile);
                             if (kb % kSFAPeriod == 0)
                                 // (split A: the two planes' words of a K-block are two rows, one box)
                                 tma_in(sfa_buffer(), &tm_sfa, sf_full_bar(stage), sfa_mn, sfa_row0 + kb / kSFAPeriod * kSFAWords * kPlanes, tile.group);
                             if (kHalfTiles && kb % kSFAPeriod == 0 && !half)       // (boxes of 64 rows)
                                 tma_in(sfa_buffer() + kSFABytes / 2, &tm_sfa, sf_full_bar(stage), sfa_mn + 64, sfa_row0 + kb / kSFAPeriod * kSFAWords * kPlanes, tile.group);
-                            if (kb % kSFBPeriod == 0)
+                            if (kb % kSFBPeriod == 0 && !asked)
                                 tma_in(sfb_buffer(), &tm_sfb, sf_full_bar(stage), tile.n_block * BLOCK_N, sfb_row0 + kb / kSFBPeriod * kSFBWords, tile.group);
                         }
                         // With a cluster the copies land in this CTA and their bytes are counted on CTA 0's barrier,
                         // which expects both CTAs' bytes
                         const uint32_t load_bar = kCluster == 1 ? full_bar(stage) : in_leader(full_bar(stage));
-                        if (kCluster == 1 || is_leader) mbar_arrive_expect_tx(full_bar(stage), kTxBytesAB - (half && !kAllHalf ? kABytes / 2 : 0u));
-                        else mbar_arrive_cluster(load_bar);
+                        if (!asked) expect_ab(stage, tile);
                         auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y) {
                             if constexpr (kL2Hint != 0 && kGemmType != kBatched) {
                                 // DG_L2_HINT 1: A stays (evict_last), B streams (evict_first); 2: the other way round
@@ -616,7 +653,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                         if constexpr (!kBMnMajor) {
                             #pragma unroll
                             for (uint32_t ka = 0; ka < kKAtoms; ++ka)
-                                load(smem_base + kSmemB + stage * kBBytes + ka * kBAtomStride, &tm_b, k_base + kb * kLoadXPerKBlock + ka * 128, b_row);
+                                if (!asked) load(smem_base + kSmemB + stage * kBBytes + ka * kBAtomStride, &tm_b, k_base + kb * kLoadXPerKBlock + ka * 128, b_row);
                         } else {
                             #pragma unroll
                             for (uint32_t i = 0; i < kBAtoms; ++i)

@@ -205,7 +205,7 @@ int launch_many_rows(const dg_gemm_args_t* g, bool ragged, const Planes& planes)
 //                splitting A for each costs more than a kernel that splits it once (N 7168 K 16384: 26 us against 21; N 4096 K 7168: 10.5 against 11.4)
 //   up to 32     the few-row kernel on A split ahead, 32 rows a pass (ragged: up to 24, a pass that a group's size leaves half empty costs
 //                as much as a full one: 320 rows in 16 groups, N 4096 K 7168: 63 us against 70 below, 400 rows 80 against 78)
-//   above        the GEMM kernel on A split ahead (48 rows, N 4096 K 7168: 13.5 us, the few-row kernel in two passes 14.6; 32 rows: 12.8 against 11.4)
+//   above        the GEMM kernel on A split ahead (48 rows, N 4096 K 7168: 12.7 us, the few-row kernel in two passes 14.6; 32 rows: 12.0 against 11.4)
 enum class Form { kSplit8, kSplit16, kPlanes16, kPlanes32, kMany };
 Form form_of(const dg_gemm_args_t* g, bool ragged) {
     const int rows = ragged ? ceil_div(g->m, g->num_groups) : g->m;
