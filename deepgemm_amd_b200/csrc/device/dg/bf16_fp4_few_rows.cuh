@@ -52,8 +52,9 @@ __device__ __forceinline__ void group_rows(const Bf16Fp4Params& p, int g, int& f
     first = 0;
     end = p.m;
     if (p.group_ends != nullptr) {
-        first = g == 0 ? 0 : min(max(p.group_ends[g - 1], 0), p.m);
-        end = min(max(p.group_ends[g], 0), p.m);
+        // (from L2: with A split ahead they are read before the kernel before this one is done)
+        first = g == 0 ? 0 : min(max(__ldcg(p.group_ends + g - 1), 0), p.m);
+        end = min(max(__ldcg(p.group_ends + g), 0), p.m);
     }
 }
 

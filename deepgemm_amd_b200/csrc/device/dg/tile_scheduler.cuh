@@ -199,7 +199,11 @@ struct TileScheduler {
             uint32_t mb = 0, rows = 0;
             while (true) {
                 if (cur_group >= num_groups) return false;
+                #if defined(__CUDA_ARCH__)
+                const int e = __ldcg(layout + cur_group);      // from L2: the producer looks before the kernel before this one is done
+#else
                 const int e = layout[cur_group];
+#endif
                 uint32_t end = e < 0 ? 0u : (static_cast<uint32_t>(e) > shape_m ? shape_m : static_cast<uint32_t>(e));
                 rows = end > group_start ? end - group_start : 0u;
                 mb = (rows + kBlockM - 1) / kBlockM;

@@ -9,6 +9,7 @@
 #include "dg_common.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 #include "device/dg/bf16_fp4_few_rows.cuh"
 
@@ -25,20 +26,89 @@ int clusters_at_once(int slices) {
     return std::max(1, kFit[slices] * dg_get_num_sms() / 148);
 }
 
-// CTAs along K (a cluster) for a launch with `items` blocks of 128 columns: the number with the fewest K-blocks in a row (~0.25 us each, an
-// SM's two CTAs side by side), a little more with partners, which finish an item before they begin the next
-int choose_slices(int64_t items, int num_blocks) {
-    int best = 1;
+// The few-row kernel's variants, and what a launch of each takes: so many us, and so many more for each K-block (128 x 128 weights) that a CTA
+// goes through, alone on its SM or next to another one.  Fitted to 374 launches of dense products of 1 to 32 rows, N x K from 512 x 4096 to
+// 7168 x 16384, in one to eight slices (4 to 95 us): half of them are met within 5 %, nine of ten within 15 %.  Splitting A costs a CTA
+// instructions for every block; A split ahead costs a kernel more.
+struct FewRows {
+    int tokens;
+    bool split;                  // splits A itself
+    double fixed, alone, beside;
+};
+constexpr double kManyRowsLeast = 7.0;       // us that the split and the GEMM take together at least
+constexpr FewRows kFewRows[] = {{8, true, 4.2, 0.275, 0.38}, {16, true, 5.3, 0.42, 0.55}, {16, false, 7.2, 0.25, 0.39}, {32, false, 6.8, 0.32, 0.49}};
+
+// How a product is computed: a variant of the few-row kernel in so many CTAs along K (a cluster), or the GEMM kernel
+struct Plan {
+    const FewRows* few;          // null: the GEMM kernel on A split ahead
+    int slices;
+};
+
+// Items of a launch: blocks of 128 columns of a group's rows, `tokens` of them at a time.  A ragged product's sizes are on the device: at most
+// one group per row and a pass more per `tokens` rows.  Expected: no two rows in one group while there are no more rows than groups;
+// above, sizes as unequal as a geometric distribution has them (c rows or more with probability q^c, q = mean / (1 + mean)), a group's passes
+// being the sum of q^(1 + j tokens).
+int64_t most_items(const dg_gemm_args_t* g, bool ragged, int tokens) {
+    const int64_t passes = ragged ? std::min(g->m, g->num_groups + g->m / tokens) : ceil_div(g->m, tokens);
+    return ceil_div(g->n, 128) * passes;
+}
+double expected_items(const dg_gemm_args_t* g, bool ragged, int tokens) {
+    double passes = ceil_div(g->m, tokens);
+    if (ragged) {
+        const double q = g->m / (static_cast<double>(g->m) + g->num_groups);
+        passes = g->m <= g->num_groups ? g->m : std::ceil(g->num_groups * q / (1.0 - std::pow(q, tokens)));
+    }
+    return ceil_div(g->n, 128) * passes;
+}
+
+Plan make_plan(const dg_gemm_args_t* g, bool ragged, int forced) {
+    const int num_blocks = g->k / 128, sms = dg_get_num_sms();
+    Plan best{nullptr, 0};
     double best_cost = 0.0;
-    for (int s = 1; s <= few::kMaxCluster && (s == 1 || num_blocks / s >= 2); ++s) {
-        const double waves = static_cast<double>(ceil_div<int64_t>(items, clusters_at_once(s)));
-        const double cost = waves * (0.25 * ceil_div(num_blocks, s) + (s > 1 ? 1.5 : 0.0));
-        if (s == 1 || cost < best_cost) {
-            best = s;
-            best_cost = cost;
+    for (const FewRows& f : kFewRows) {
+        if (forced >= 1 && forced <= 4 && &f != &kFewRows[forced - 1]) continue;
+        const double items = expected_items(g, ragged, f.tokens);
+        for (int s = 1; s <= few::kMaxCluster && (s == 1 || num_blocks / s >= 2); ++s) {
+            // (CTAs that take many items do not keep step: half an item more than the average then, not a whole one)
+            const double at_once = clusters_at_once(s), waves = items <= 2 * at_once ? std::ceil(items / at_once) : items / at_once + 0.5;
+            const bool beside = std::min(items, at_once) * s > sms;
+            // (partners finish an item before they begin the next)
+            const double cost = f.fixed + waves * ceil_div(num_blocks, s) * (beside ? f.beside : f.alone) + (waves - 1) * (s > 1 ? 2.0 : 0.5);
+            if (best.few == nullptr || cost < best_cost) {
+                best = Plan{&f, s};
+                best_cost = cost;
+            }
         }
     }
+    // The GEMM kernel has tiles of 64 or 128 rows of A, this one 128 columns of D and as many rows as there are: by the rows that meet one
+    // matrix of weights (ragged: the average group; a pass that a group leaves half empty costs as much as a full one).  48 rows, N 4096
+    // K 7168: 12.7 us, the few-row kernel 14.6; 32 rows 12.0 against 11.4; 320 rows in 16 groups 70 against 63, 400 rows 78 against 80.  Where the weights are
+    // few, two launches cost more than the passes (64 rows, N 1024 K 1024: 5.7 us against 6.3).
+    const int rows = ragged ? ceil_div(g->m, g->num_groups) : g->m;
+    // (it stores whole 16-byte pieces of a row of D: where N ends inside one, what follows the row would not stay)
+    const int d_elem = g->d_dtype == DG_FP32 ? 4 : 2;
+    const bool many = forced ? forced == 5 : rows > (ragged ? 24 : 32) && best_cost > kManyRowsLeast;
+    if (many && (static_cast<int64_t>(g->n) * d_elem) % 16 == 0) best = Plan{nullptr, 0};
     return best;
+}
+
+// The last sizes' plan is kept: the question is asked twice a call, and a small product takes the GPU no longer than the host
+Plan plan_of(const dg_gemm_args_t* g, bool ragged) {
+    struct Sizes {
+        int m, n, k, groups, d_dtype, ragged, sms, forced;
+        bool operator==(const Sizes& o) const {
+            return m == o.m && n == o.n && k == o.k && groups == o.groups && d_dtype == o.d_dtype && ragged == o.ragged && sms == o.sms && forced == o.forced;
+        }
+    };
+    thread_local Sizes last{};
+    thread_local Plan plan{};
+    // DG_FORCE_BF16_FP4_FORM: 1-4: the variants above in their order, 5: the GEMM kernel
+    const Sizes now{g->m, g->n, g->k, g->num_groups, static_cast<int>(g->d_dtype), ragged, dg_get_num_sms(), env_int("FORCE_BF16_FP4_FORM")};
+    if (!(now == last)) {
+        plan = make_plan(g, ragged, now.forced);
+        last = now;
+    }
+    return plan;
 }
 
 // A split ahead of the product: [hi, lo][slot][k] E4M3 bytes, then their scale words [k / 128][hi, lo][slot] (four UE8M0 codes, one per 32
@@ -55,39 +125,43 @@ constexpr int kSplitRows = 16, kSplitCols = 512;
 
 // One CTA splits 16 rows x 512 columns: 16-byte loads, quads of lanes share a scale, 8-byte stores, and the scale words of the 16 rows leave
 // together (they are neighbours when the rows are).  Bound by memory: 2 bytes in, 2 + 1/16 out per element.
-__global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* __restrict__ a, int64_t lda, const Planes out, int m, int k,
-                                                         const int* __restrict__ group_ends, int groups) {
+__global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* a, int64_t lda, const Planes out, int m, int k, const int* group_ends, int groups) {
     __shared__ int slot_of[kSplitRows];
     __shared__ uint32_t words[2][kSplitCols / 128][kSplitRows];
     // (in this order: what the product's kernel reads before it waits for this one, the weights, is then complete as well)
     griddep_wait();
     griddep_launch_dependents();
     const int row0 = blockIdx.x * kSplitRows, r = threadIdx.x / 16, chunk = threadIdx.x % 16, row = row0 + r;
-    if (threadIdx.x < kSplitRows) {
-        const int mine = row0 + threadIdx.x;
-        int slot = mine < m ? mine : -1;
-        if (group_ends != nullptr && slot >= 0) {
-            // the group that holds the row: the first whose end lies behind it
-            int lo = 0, hi = groups;
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                if (group_ends[mid] > mine) hi = mid;
-                else lo = mid + 1;
-            }
-            const int first = lo == 0 ? 0 : min(max(group_ends[lo - 1], 0), m);
-            slot = lo == groups ? -1 : first_slot(first, lo) + mine - first;
-        }
-        slot_of[threadIdx.x] = slot;
-    }
-    __syncthreads();
-    const int slot = slot_of[r];
     uint4 raw[kSplitCols / 128];
     #pragma unroll
     for (int b = 0; b < kSplitCols / 128; ++b) {
         const int col = blockIdx.y * kSplitCols + b * 128 + chunk * 8;
         raw[b] = make_uint4(0, 0, 0, 0);
-        if (slot >= 0 && col < k) raw[b] = __ldg(reinterpret_cast<const uint4*>(a + row * lda + col));
+        // (from L2: this kernel was there before its predecessor had written A, so not through the read-only path)
+        if (row < m && col < k) raw[b] = __ldcg(reinterpret_cast<const uint4*>(a + row * lda + col));
     }
+    // Meanwhile the first warp finds the rows' slots: a row's group is the number of ends at or before it
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x, mine = row0 + lane;
+        int group = 0, first = 0;
+        if (group_ends != nullptr) {
+            for (int g0 = 0; g0 < groups; g0 += 32) {
+                const int end = g0 + lane < groups ? min(max(__ldcg(group_ends + g0 + lane), 0), m) : INT32_MAX;
+                #pragma unroll
+                for (int i = 0; i < kSplitRows; ++i) {
+                    const int behind = __popc(__ballot_sync(0xFFFFFFFFu, end <= row0 + i));
+                    const int last = __shfl_sync(0xFFFFFFFFu, end, max(behind - 1, 0));
+                    if (lane == i && behind > 0) {
+                        group += behind;
+                        first = last;
+                    }
+                }
+            }
+        }
+        if (lane < kSplitRows) slot_of[lane] = mine >= m || (group_ends != nullptr && group >= groups) ? -1 : group_ends != nullptr ? first_slot(first, group) + mine - first : mine;
+    }
+    __syncthreads();
+    const int slot = slot_of[r];
     uint2 hi[kSplitCols / 128], lo[kSplitCols / 128];
     uint32_t code[kSplitCols / 128];
     split_bf16<kSplitCols / 128>(raw, hi, lo, code);
@@ -137,12 +211,9 @@ int split_rows(const dg_gemm_args_t* g, const int* group_ends, const Planes& pla
 }
 
 template <int kTokens, bool kSplit>
-int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Planes& planes) {
+int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Planes& planes, int slices) {
     using S = few::Shape<kTokens, kSplit>;
-    // Items: exact for a dense product; a ragged one has at most one group per row, and a pass more per kTokens rows
-    const int64_t tiles_n = ceil_div(g->n, 128), passes = ceil_div(g->m, kTokens);
-    const int64_t items = tiles_n * (p.group_ends != nullptr ? std::min(g->m, g->num_groups + g->m / kTokens) : passes);
-    const int slices = choose_slices(items, g->k / 128);
+    const int64_t items = most_items(g, p.group_ends != nullptr, kTokens);
     CUtensorMap tm_w, tm_sf, tm_a, tm_sfa;
     int rc;
     const uint64_t words = ceil_div(g->k, 4 * g->gran_k_b);
@@ -198,37 +269,14 @@ int launch_many_rows(const dg_gemm_args_t* g, bool ragged, const Planes& planes)
     return run_split_a_gemm(&args, ragged, planes.slots);
 }
 
-// Which kernels a product takes, by the rows of A that meet one matrix of weights (ragged: on average; the sizes are on the device):
-//   up to 8      the few-row kernel, splitting A itself; with more weights than below, and groups that hold more than 8 rows as often as not,
-//                16 rows a pass on A split ahead (131 rows in 32 groups, N 7168 K 2048: 40 us against 49)
-//   up to 16     the same with 16 rows a pass, as long as an SM has no more than ~16 blocks of 128 x 128 weights to go through; with more of them
-//                splitting A for each costs more than a kernel that splits it once (N 7168 K 16384: 26 us against 21; N 4096 K 7168: 10.5 against 11.4)
-//   up to 32     the few-row kernel on A split ahead, 32 rows a pass (ragged: up to 24, a pass that a group's size leaves half empty costs
-//                as much as a full one: 320 rows in 16 groups, N 4096 K 7168: 63 us against 70 below, 400 rows 80 against 78)
-//   above        the GEMM kernel on A split ahead (48 rows, N 4096 K 7168: 12.7 us, the few-row kernel in two passes 14.6; 32 rows: 12.0 against 11.4)
-enum class Form { kSplit8, kSplit16, kPlanes16, kPlanes32, kMany };
-Form form_of(const dg_gemm_args_t* g, bool ragged) {
-    const int rows = ragged ? ceil_div(g->m, g->num_groups) : g->m;
-    const int64_t blocks = static_cast<int64_t>(ceil_div(g->n, 128)) * ceil_div(g->k, 128) * (ragged ? std::min(g->num_groups, g->m) : 1);
-    const bool many_blocks = blocks > static_cast<int64_t>(16) * dg_get_num_sms();
-    if (rows <= 8 && !(ragged && rows > 4 && many_blocks)) return Form::kSplit8;
-    if (rows <= 16) return many_blocks ? Form::kPlanes16 : Form::kSplit16;
-    // (the GEMM kernel stores whole 16-byte pieces of a row of D: where N ends inside one, what follows the row would not stay)
-    const int d_elem = g->d_dtype == DG_FP32 ? 4 : 2;
-    return rows <= (ragged ? 24 : 32) || (static_cast<int64_t>(g->n) * d_elem) % 16 != 0 ? Form::kPlanes32 : Form::kMany;
-}
-bool splits_inside(const dg_gemm_args_t* g, bool ragged) {
-    const Form form = form_of(g, ragged);
-    return form == Form::kSplit8 || form == Form::kSplit16;
-}
-
-size_t workspace_bytes(const dg_gemm_args_t* g, bool ragged) {
-    return g->m == 0 || g->n == 0 || splits_inside(g, ragged) ? 0 : planes_bytes(num_slots(g->m, g->num_groups, ragged), g->k);
+size_t workspace_bytes(const dg_gemm_args_t* g, bool ragged, const Plan& plan) {
+    return plan.few != nullptr && plan.few->split ? 0 : planes_bytes(num_slots(g->m, g->num_groups, ragged), g->k);
 }
 
 int run(const dg_gemm_args_t* g, bool ragged, void* workspace, int64_t given_bytes) {
     DG_REQUIRE_ALIVE();
     DG_REQUIRE(g != nullptr);
+    env_refresh();
     DG_REQUIRE(g->a_dtype == DG_BF16 && g->b_dtype == DG_FP4_E2M1_X2);
     DG_REQUIRE(g->d_dtype == DG_BF16 || (g->d_dtype == DG_FP32 && !ragged));
     DG_REQUIRE(g->major_a == DG_MAJOR_K && g->major_b == DG_MAJOR_K);
@@ -250,7 +298,8 @@ int run(const dg_gemm_args_t* g, bool ragged, void* workspace, int64_t given_byt
     DG_REQUIRE(g->ldd >= g->n && (g->ldd * d_elem) % 16 == 0);
     DG_REQUIRE(g->sfb_pitch >= align_up<int64_t>(g->n, 4) && g->sfb_pitch % 4 == 0);
 
-    const size_t needed = workspace_bytes(g, ragged);
+    const Plan plan = plan_of(g, ragged);
+    const size_t needed = workspace_bytes(g, ragged, plan);
     DG_REQUIRE(needed == 0 || (workspace != nullptr && aligned(workspace, 128) && given_bytes >= 0 && static_cast<size_t>(given_bytes) >= needed));
     int rc = ensure_status_word();
     if (rc != DG_OK) return rc;
@@ -258,21 +307,19 @@ int run(const dg_gemm_args_t* g, bool ragged, void* workspace, int64_t given_byt
     const Planes planes{static_cast<uint8_t*>(workspace), reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + static_cast<size_t>(2) * slots * g->k), slots};
     const Bf16Fp4Params p{g->d, ragged ? g->grouped_layout : nullptr, state().status_device, g->m, g->n, g->k, g->ldd, g->d_dtype == DG_FP32,
                           g->accumulate != 0, g->has_alpha ? g->alpha : 1.0f, slots, g->num_groups};
-    switch (form_of(g, ragged)) {
-        case Form::kSplit8: return launch_few_rows<8, true>(g, p, planes);
-        case Form::kSplit16: return launch_few_rows<16, true>(g, p, planes);
-        case Form::kPlanes16: return launch_few_rows<16, false>(g, p, planes);
-        case Form::kPlanes32: return launch_few_rows<32, false>(g, p, planes);
-        case Form::kMany: break;
-    }
-    return launch_many_rows(g, ragged, planes);
+    if (plan.few == nullptr) return launch_many_rows(g, ragged, planes);
+    if (plan.few->split) return plan.few->tokens == 8 ? launch_few_rows<8, true>(g, p, planes, plan.slices) : launch_few_rows<16, true>(g, p, planes, plan.slices);
+    return plan.few->tokens == 16 ? launch_few_rows<16, false>(g, p, planes, plan.slices) : launch_few_rows<32, false>(g, p, planes, plan.slices);
 }
 
 }  // namespace
 }  // namespace dg
 
 extern "C" int64_t dg_bf16_fp4_workspace_bytes(const dg_gemm_args_t* args, int ragged) {
-    return args == nullptr || args->m < 0 || args->k < 0 || args->num_groups <= 0 ? -1 : static_cast<int64_t>(dg::workspace_bytes(args, ragged != 0));
+    dg::env_refresh();
+    if (args == nullptr || args->m < 0 || args->n < 0 || args->k < 0 || args->num_groups <= 0) return -1;
+    if (args->m == 0 || args->n == 0 || args->k == 0) return 0;
+    return static_cast<int64_t>(dg::workspace_bytes(args, ragged != 0, dg::plan_of(args, ragged != 0)));
 }
 extern "C" int dg_bf16_fp4_gemm(const dg_gemm_args_t* args, void* workspace, int64_t workspace_bytes) { return dg::run(args, false, workspace, workspace_bytes); }
 extern "C" int dg_m_grouped_bf16_fp4_gemm_ragged(const dg_gemm_args_t* args, void* workspace, int64_t workspace_bytes) {

@@ -229,7 +229,7 @@ DG_API int dg_fp8_bmm(const dg_gemm_args_t* args);
  * groups and no alignment; ends must not decrease; rows at or behind the last end are not written.
  * Sums are FP32, one rounding per element of D.  A row of A with an infinity or a NaN gives non-finite results.
  * workspace: device memory of this call alone until it has completed, 128-byte aligned, at least
- * dg_bf16_fp4_workspace_bytes(args, ragged) bytes (0 for a few rows per matrix of weights, about 2 m k above; it reads only the
+ * dg_bf16_fp4_workspace_bytes(args, ragged) bytes (0 for a few rows or weights, about 2 m k above; it reads only the
  * sizes, num_groups and d_dtype in args; -1: no valid sizes). */
 DG_API int64_t dg_bf16_fp4_workspace_bytes(const dg_gemm_args_t* args, int ragged);
 DG_API int dg_bf16_fp4_gemm(const dg_gemm_args_t* args, void* workspace_device, int64_t workspace_bytes);

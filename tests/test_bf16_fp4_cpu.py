@@ -60,12 +60,13 @@ def test_python_functions_refuse_cpu_tensors_and_wrong_shapes():
 
 def test_workspace():
     size = lambda ragged=0, **kw: _lib.lib.dg_bf16_fp4_workspace_bytes(C.byref(args(**kw)), ragged)  # noqa: E731
-    assert size(m=8) == 0 and size(m=0) == 0 and size(m=24, num_groups=3, ragged=1) == 0
-    assert size(m=101) == 2 * 104 * (256 + 8)                                  # two planes of E4M3 and a scale per 32 of them, rows in fours
-    assert size(m=101, num_groups=3, ragged=1) >= 2 * (101 + 3 * 3) * (256 + 8)        # every group starts on a multiple of four
+    big = dict(n=4096, k=4096, ldb=2048, sfb_pitch=4096)
+    assert size(m=8) == 0 and size(m=0) == 0 and size(m=24, num_groups=3, ragged=1) == 0 and size(m=1, **big) == 0
+    assert size(m=101, **big) == 2 * 104 * (4096 + 128)                        # two planes of E4M3 and a scale per 32 of them, rows in fours
+    assert size(m=101, num_groups=3, ragged=1, **big) >= 2 * (101 + 3 * 3) * (4096 + 128)        # every group starts on a multiple of four
     assert _lib.lib.dg_bf16_fp4_workspace_bytes(None, 0) == -1 and size(m=-1) == -1 and size(num_groups=0, ragged=1) == -1
     for kw in (dict(workspace=None), dict(workspace=0x7000, given=100), dict(workspace=0x7040), dict(workspace=0x7000, given=-1)):
-        assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(m=64)), kw.get("workspace"), kw.get("given", 1 << 20)) != _lib.DG_OK
+        assert _lib.lib.dg_bf16_fp4_gemm(C.byref(args(m=64, lda=4096, ldd=4096, **big)), kw.get("workspace"), kw.get("given", 1 << 24)) != _lib.DG_OK
         assert "workspace" in _lib.last_error()
 
 

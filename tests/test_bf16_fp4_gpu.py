@@ -24,6 +24,14 @@ pytestmark = pytest.mark.gpu
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
 
 
+@pytest.fixture(params=[0, 1, 2, 3, 4, 5], ids=["chosen", "8", "16", "16-ahead", "32-ahead", "gemm"])
+def form(request, monkeypatch):
+    """The ways a product is computed, each of them at every size: 8 or 16 rows a pass split inside the kernel, 16 or 32 split ahead, the GEMM kernel."""
+    if request.param:
+        monkeypatch.setenv("DG_FORCE_BF16_FP4_FORM", str(request.param))
+    return request.param
+
+
 def pack_scales(exps, mn_pad=0):
     """UE8M0 codes [G?, n, blocks] -> packed int32 [G?, n, ceil(blocks / 4)], MN-major with pitch align(n, 4) + mn_pad."""
     lead, (n, blocks) = exps.shape[:-2], exps.shape[-2:]
@@ -86,6 +94,7 @@ DENSE = [(1, 8, 128), (1, 2112, 7168), (1, 264, 16384), (2, 24, 256), (5, 100, 3
          (40, 96, 256), (127, 128, 3200), (192, 1544, 256), (193, 264, 1024), (128, 2112, 512), (129, 256, 512), (300, 1000, 768), (511, 136, 128), (1030, 520, 384), (2500, 1032, 1280)]
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("m,n,k", DENSE)
 @pytest.mark.parametrize("gran,out", [(32, torch.bfloat16), (128, torch.float)])
 def test_dense(m, n, k, gran, out):
@@ -100,6 +109,7 @@ def test_dense(m, n, k, gran, out):
     assert dg.kernel_status() == 0
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("m", [1, 6, 14, 40, 64, 150, 200, 600])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float])
 @pytest.mark.parametrize("in_place", [True, False])
@@ -113,6 +123,7 @@ def test_dense_accumulates_and_scales(m, out, in_place):
     check_product(d, a, w, added=c, alpha=float(torch.tensor(-0.37)))
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("m", [1, 3, 24, 90, 400])
 @pytest.mark.parametrize("gran", [32, 128])
 def test_padded_pitches_and_odd_columns(m, gran):
@@ -129,6 +140,7 @@ def test_padded_pitches_and_odd_columns(m, gran):
     assert (wide_d[:, n:] == -7.0).all()
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("m", [1, 8, 32, 70, 300])
 def test_wide_ranges_of_activations_and_scales(m):
     """Rows from 2^-100 to 2^60, elements of one row 2^20 apart, rows and blocks of zeros, scale codes 0 and far apart."""
@@ -147,6 +159,7 @@ def test_wide_ranges_of_activations_and_scales(m):
     check_product(d, a, w)
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("m", [4, 48, 260])
 def test_rows_that_are_not_finite_stay_among_themselves(m):
     n, k = 264, 512
@@ -191,6 +204,7 @@ def check_ragged(d, a, w, counts, untouched):
     assert (d[start:] == untouched).all()
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("counts,spare", RAGGED)
 @pytest.mark.parametrize("n,k,gran", [(264, 640, 32), (1096, 1536, 128)])
 def test_ragged(counts, spare, n, k, gran):
@@ -201,6 +215,7 @@ def test_ragged(counts, spare, n, k, gran):
     assert dg.kernel_status() == 0
 
 
+@pytest.mark.usefixtures("form")
 def test_ragged_padded_pitches():
     counts, n, k = [3, 0, 70, 5], 136, 256
     codes, e, w, a, ends = ragged_case(counts, 3, n, k, 32, 30)
@@ -215,6 +230,7 @@ def test_ragged_padded_pitches():
         assert (wide_d[:, n:] == -7.0).all()
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("rows", [24, 700])
 def test_ragged_ends_outside_the_rows_are_clipped(rows):
     """Ends beyond the rows of A, below zero or going back make groups shorter or empty and write nothing outside D."""
@@ -228,6 +244,7 @@ def test_ragged_ends_outside_the_rows_are_clipped(rows):
     check_product(d[5:], a[5:], w[3])
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("rows", [40, 900])
 def test_ragged_graph_replays_follow_the_ends(rows):
     n, k, groups = 264, 512, 6
@@ -248,6 +265,7 @@ def test_ragged_graph_replays_follow_the_ends(rows):
         check_ragged(d, a, w, counts, -7.0)
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("m", [4, 300])
 def test_two_streams_and_two_graphs_at_once(m):
     """Calls in flight together share nothing: two streams, then two graphs captured apart and replayed side by side."""
@@ -279,10 +297,11 @@ def test_two_streams_and_two_graphs_at_once(m):
         check_product(s["d"], s["a"], s["w"])
 
 
-FORMS = [1, 8, 14, 24, 48, 200]                    # rows of A: one count for each way a dense product is computed
-RAGGED_FORMS = [3, 7, 12, 20, 40, 150]             # ... rows of an average group
+FORMS = [1, 14, 48, 200]                           # rows of A
+RAGGED_FORMS = [3, 12, 40, 150]                    # ... of an average group
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("average", RAGGED_FORMS)
 @pytest.mark.parametrize("groups", [33, 300])
 def test_many_groups(groups, average):
@@ -300,6 +319,7 @@ def test_many_groups(groups, average):
     assert dg.kernel_status() == 0
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("n,k,gran", [(4096, 2176, 128), (136, 16384, 32), (20000, 256, 32)])
 @pytest.mark.parametrize("m", FORMS)
 def test_slices_and_passes_of_every_form(m, n, k, gran):
@@ -311,6 +331,7 @@ def test_slices_and_passes_of_every_form(m, n, k, gran):
     check_product(d, a, w)
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("captured", [False, True])
 @pytest.mark.parametrize("m", FORMS)
 def test_operands_written_just_before_and_read_just_after(m, captured):
@@ -345,6 +366,7 @@ def test_operands_written_just_before_and_read_just_after(m, captured):
     check_product(last, mid, w1)
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("average", RAGGED_FORMS)
 def test_ends_written_just_before(average):
     groups, n, k = 40, 520, 512
@@ -364,6 +386,7 @@ def test_ends_written_just_before(average):
         check_ragged(d, a, w, counts.tolist(), -7.0)
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("average", RAGGED_FORMS)
 def test_ragged_calls_in_flight_together(average):
     groups, n, k = 12, 1024, 768
@@ -383,6 +406,7 @@ def test_ragged_calls_in_flight_together(average):
         check_ragged(s["args"][2], s["args"][0], s["w"], s["counts"], -7.0)
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("m", FORMS)
 def test_the_compiled_binding_and_the_ctypes_one_give_the_same_bits(m, monkeypatch):
     n, k, groups = 520, 1152, 3
@@ -402,6 +426,7 @@ def test_the_compiled_binding_and_the_ctypes_one_give_the_same_bits(m, monkeypat
     assert all(torch.equal(x, y) for x, y in zip(got[:3], got[3:]))
 
 
+@pytest.mark.usefixtures("form")
 def test_more_than_a_million_rows():
     m, n, k = 1_100_001, 24, 128
     codes, e, w = make_weights((n, k), 32, 150)
@@ -437,6 +462,7 @@ def test_outputs_beyond_32_bit_offsets():
     assert dg.kernel_status() == 0
 
 
+@pytest.mark.usefixtures("form")
 @pytest.mark.parametrize("tokens", [1, 13, 160])
 def test_an_expert_layer_end_to_end(tokens):
     """A projection, the routed rows sorted by expert, the two expert products around a gated activation, and the weighted sum
