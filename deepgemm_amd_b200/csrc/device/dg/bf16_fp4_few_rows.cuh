@@ -14,7 +14,7 @@
 // Work.  W is the 128-row operand: an item is 128 columns of D times up to kTokens rows of A (2 kTokens tile columns).  CTAs stay and take
 // items in turn; the accumulators are double, so an item's epilogue runs under the next one's loads and products.
 //   warp 0      TMA producer: per 128 elements of K 128 rows of W (8 KB, unpacked to a byte each on the way), their scale words, and A
-//   warp 1      MMA issuer
+//   warps 1, 3  MMA issuers (narrow tiles: both, taking K-blocks in turn; their accumulators are added at the end)
 //   warp 2      allocates tensor memory, rearranges scale words for tcgen05.cp
 //   warps 4-7   epilogue
 //   warps 8-15  in teams of two: split a stage's rows of A into its tile columns and their scales.  For more rows, or more weights to a
@@ -185,7 +185,12 @@ template <int kTokens, bool kSplit> struct Shape {
     static_assert(!kSplit || (kTokens <= 16 && kTeams <= kStages), "a team that is done with its last block knows that the stage of its next one is at most one block behind");
     static constexpr int kOffB = kStages * 16384, kOffA = kOffB + kStages * kCols * 128, kOffSfa = kOffA + (kSplit ? kStages * kTokens * 256 : 0), kOffSfb = kOffSfa + kStages * 512;
     static constexpr int kOffBar = kOffSfb + kStages * 512, kOffMisc = kOffBar + (4 * kStages + 4) * 8, kOffRecv = (kOffMisc + 8 + 15) / 16 * 16;
-    static constexpr int kTmemCols = 2 * kCols + 8 <= 64 ? 64 : (2 * kCols + 8 <= 128 ? 128 : 256);
+    // MMA-issuing warps, taking K-blocks in turn: with tiles this narrow a warp's walk around its loop takes 550 cycles, the MMAs 100.  Each
+    // has accumulators and scale columns of its own (what two threads issue has no order).  (7 rows, N 24576 K 1536: 8.6 -> 8.2 us; 131 rows in
+    // 32 groups of N 7168 K 2048, 8 a pass: 43 -> 40.  16 rows split inside are bound by the splitting, 32 by the MMAs)
+    static constexpr int kIssuers = kTokens * (kSplit ? 2 : 1) <= 16 ? 2 : 1;
+    static constexpr int kScaleCol = 2 * kIssuers * kCols, kTmemUsed = kScaleCol + 8 * kIssuers;
+    static constexpr int kTmemCols = kTmemUsed <= 64 ? 64 : (kTmemUsed <= 128 ? 128 : 256);
     static_assert(kTokens <= 32, "two CTAs' shares of an SM's shared and tensor memory");
     // What a CTA receives: every slice's partial sums of the rows of D it owns
     __host__ __device__ static constexpr int recv_rows(int slices) { return (kTokens + slices - 1) / slices; }
@@ -259,7 +264,7 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                 mbar_init(a_bar(s), 1);
             }
             for (uint32_t a = 0; a < 2; ++a) {
-                mbar_init(done_bar(a), 1);       // tcgen05.commit: an item's accumulators are complete
+                mbar_init(done_bar(a), S::kIssuers);       // tcgen05.commit: an item's accumulators are complete
                 mbar_init(free_bar(a), 4);       // the epilogue warps have read them
             }
             fence_mbar_init();
@@ -284,7 +289,8 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem = __reduce_max_sync(0xFFFFFFFFu, *tmem_slot), tmem_sfa = tmem + 2 * kCols, tmem_sfb = tmem_sfa + 4;
+    const uint32_t tmem = __reduce_max_sync(0xFFFFFFFFu, *tmem_slot);
+    auto accumulators = [&](uint32_t a, uint32_t issuer) { return tmem + (a * S::kIssuers + issuer) * kCols; };
     griddep_wait();
     griddep_launch_dependents();
     bool ok = true;
@@ -310,13 +316,21 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                 }
                 __syncwarp();
             }
-        } else if (warp == 1) {
+        } else if (warp == 1 || (S::kIssuers == 2 && warp == 3)) {
             constexpr uint32_t idesc = make_instr_desc_block_scaled(kFmtE2M1, kFmtE4M3, 0, 0, 128, kCols);
+            const int me = warp == 1 ? 0 : 1, blocks = kb1 - kb0;
+            const uint32_t tmem_d = accumulators(accum, me), tmem_sfa = tmem + S::kScaleCol + 8 * me, tmem_sfb = tmem_sfa + 4;
             if (some) ok = ok && warp_wait(free_bar(accum), accum_phase ^ 1, ctx, 2);
             tc_fence_after_sync();
-            for (int kb = kb0; ok && kb < kb1; ++kb, advance()) {
+            if (some && me >= blocks && lane == 0) mbar_arrive(done_bar(accum));       // (nothing to do for the second one)
+            for (int b = 0; ok && b < blocks; ++b, advance()) {
+                if (b % S::kIssuers != me) continue;
+                // First that the stage's block before this one, perhaps the other warp's, has been multiplied (a barrier two phases behind answers
+                // like one that is done)
+                if (S::kIssuers > 1 && !(ok = warp_wait(empty_bar(stage), phase ^ 1, ctx, 2))) break;
                 if (!(ok = warp_wait(full_bar(stage), phase, ctx, 2))) break;
                 tc_fence_after_sync();
+                const int kb = kb0 + b;
                 const uint64_t a_desc = make_smem_desc(base + stage * 16384, 0, 1024, kSwizzle128B);
                 const uint64_t b_desc = make_smem_desc(base + S::kOffB + stage * kCols * 128, 0, 1024, kSwizzle128B);
                 const uint64_t sfa_desc = make_smem_desc(base + S::kOffSfa + stage * 512, 0, 128, kSwizzleNone);
@@ -326,10 +340,10 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
                     tc_cp_32x128b_warpx4<1>(tmem_sfb, sfb_desc);
                     #pragma unroll
                     for (uint32_t j = 0; j < 4; ++j)
-                        tc_mma_mxf8f6f4<1>(tmem + accum * kCols, a_desc + j * 2, b_desc + j * 2, instr_desc_with_sf_ids(idesc, kGran == 32 ? j : kb % 4, j),
-                                           tmem_sfa, tmem_sfb, kb != kb0 || j != 0);
+                        tc_mma_mxf8f6f4<1>(tmem_d, a_desc + j * 2, b_desc + j * 2, instr_desc_with_sf_ids(idesc, kGran == 32 ? j : kb % 4, j),
+                                           tmem_sfa, tmem_sfb, b != me || j != 0);
                     tc_commit(empty_bar(stage));
-                    if (kb + 1 == kb1) tc_commit(done_bar(accum));
+                    if (b + S::kIssuers >= blocks) tc_commit(done_bar(accum));
                 }
                 __syncwarp();
             }
@@ -430,15 +444,23 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
             float y[kTokens];
             #pragma unroll
             for (int t0 = 0; t0 < kTokens; t0 += 16) {
+                // columns hi, lo of 16 rows (of 8: both in one load), the second issuer's added to the first's
                 uint32_t v[16], w[16];
-                if (some) {
-                    tmem_ld_32x32b_x16(tmem + ((quarter * 32) << 16) + accum * kCols + t0, v);
-                    if constexpr (kTokens >= 16) tmem_ld_32x32b_x16(tmem + ((quarter * 32) << 16) + accum * kCols + kTokens + t0, w);
-                    tmem_ld_wait();
-                }
                 #pragma unroll
-                for (int i = 0; i < (kTokens < 16 ? kTokens : 16); ++i)
-                    y[t0 + i] = !some ? 0.0f : __uint_as_float(v[i]) + __uint_as_float(kTokens >= 16 ? w[i] : v[i + 8]);
+                for (int issuer = 0; issuer < S::kIssuers; ++issuer) {
+                    const bool mine = kb1 - kb0 > issuer;
+                    if (mine) {
+                        const uint32_t from = ((quarter * 32) << 16) + accumulators(accum, issuer) + t0;
+                        tmem_ld_32x32b_x16(from, v);
+                        if constexpr (kTokens >= 16) tmem_ld_32x32b_x16(from + kTokens, w);
+                        tmem_ld_wait();
+                    }
+                    #pragma unroll
+                    for (int i = 0; i < (kTokens < 16 ? kTokens : 16); ++i) {
+                        const float sum = !mine ? 0.0f : __uint_as_float(v[i]) + __uint_as_float(kTokens >= 16 ? w[i] : v[i + 8]);
+                        y[t0 + i] = issuer == 0 ? sum : y[t0 + i] + sum;
+                    }
+                }
             }
             if (some) {
                 tc_fence_before_sync();

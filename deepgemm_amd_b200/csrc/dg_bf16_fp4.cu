@@ -27,16 +27,16 @@ int clusters_at_once(int slices) {
 }
 
 // The few-row kernel's variants, and what a launch of each takes: so many us, and so many more for each K-block (128 x 128 weights) that a CTA
-// goes through, alone on its SM or next to another one.  Fitted to 374 launches of dense products of 1 to 32 rows, N x K from 512 x 4096 to
-// 7168 x 16384, in one to eight slices (4 to 95 us): half of them are met within 5 %, nine of ten within 15 %.  Splitting A costs a CTA
-// instructions for every block; A split ahead costs a kernel more.
+// goes through, alone on its SM or next to another one.  Fitted to 265 launches of dense products of 1 to 64 rows, N x K from 512 x 4096 to
+// 7168 x 16384, in one to eight slices (4 to 95 us): half of them are met within 5 %, nine of ten within 13 %.  Splitting A costs a CTA
+// instructions for every block (1 row 0.33 us, 8 rows 0.37); A split ahead costs a kernel more (0.8 us outside of a graph, half of it counted).
 struct FewRows {
     int tokens;
     bool split;                  // splits A itself
     double fixed, alone, beside;
 };
 constexpr double kManyRowsLeast = 7.0;       // us that the split and the GEMM take together at least
-constexpr FewRows kFewRows[] = {{8, true, 4.2, 0.275, 0.38}, {16, true, 5.3, 0.42, 0.55}, {16, false, 7.2, 0.25, 0.39}, {32, false, 6.8, 0.32, 0.49}};
+constexpr FewRows kFewRows[] = {{8, true, 4.2, 0.23, 0.37}, {16, true, 6.0, 0.36, 0.48}, {16, false, 6.3, 0.27, 0.39}, {32, false, 7.0, 0.325, 0.45}};
 
 // How a product is computed: a variant of the few-row kernel in so many CTAs along K (a cluster), or the GEMM kernel
 struct Plan {
@@ -73,7 +73,7 @@ Plan make_plan(const dg_gemm_args_t* g, bool ragged, int forced) {
             const double at_once = clusters_at_once(s), waves = items <= 2 * at_once ? std::ceil(items / at_once) : items / at_once + 0.5;
             const bool beside = std::min(items, at_once) * s > sms;
             // (partners finish an item before they begin the next)
-            const double cost = f.fixed + waves * ceil_div(num_blocks, s) * (beside ? f.beside : f.alone) + (waves - 1) * (s > 1 ? 2.0 : 0.5);
+            const double cost = f.fixed + waves * ceil_div(num_blocks, s) * (beside ? f.beside : f.alone) + (waves - 1) * (s > 1 ? 2.5 : 0.3);
             if (best.few == nullptr || cost < best_cost) {
                 best = Plan{&f, s};
                 best_cost = cost;
