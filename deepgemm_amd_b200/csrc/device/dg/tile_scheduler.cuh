@@ -199,7 +199,7 @@ struct TileScheduler {
             uint32_t mb = 0, rows = 0;
             while (true) {
                 if (cur_group >= num_groups) return false;
-                #if defined(__CUDA_ARCH__)
+#if defined(__CUDA_ARCH__)
                 const int e = __ldcg(layout + cur_group);      // from L2: the producer looks before the kernel before this one is done
 #else
                 const int e = layout[cur_group];

@@ -436,6 +436,43 @@ def test_more_than_a_million_rows():
     check_product(d, a, w)
 
 
+@pytest.mark.usefixtures("form")
+@pytest.mark.parametrize("captured", [False, True])
+def test_behind_a_memset_a_copy_and_a_join_of_two_streams(captured):
+    """What comes before a product is not always one kernel."""
+    m, n, k = 20, 1024, 768
+    codes, e, w = make_weights((n, k), 32, 160)
+    b, a0, host = (codes, pack_scales(e)), make_rows(m, k, 161), make_rows(m, k, 162).cpu().pin_memory()
+    a, d, d2, d3 = torch.empty_like(a0), *(torch.empty((m, n), dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    side = torch.cuda.Stream()
+    dg.bf16_fp4_gemm_nt(a0, b, d)
+
+    def run():
+        main = torch.cuda.current_stream()
+        a.copy_(host, non_blocking=True)
+        dg.bf16_fp4_gemm_nt(a, b, d)                    # behind a copy from the host
+        d2.zero_()
+        dg.bf16_fp4_gemm_nt(a, b, d2, c=d2)             # behind a memset
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            a.copy_(a0)
+            d3.fill_(1.0)
+        d2.add_(1.0)
+        main.wait_stream(side)
+        dg.bf16_fp4_gemm_nt(a, b, d3, c=d3)             # behind two streams' work
+
+    torch.cuda.synchronize()
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+    for _ in range(5):
+        graph.replay() if captured else run()
+    torch.cuda.synchronize()
+    check_product(d, host.cuda(), w)
+    check_product(d3, a0, w, added=torch.ones_like(d3))
+
+
 def test_weights_beyond_32_bit_offsets():
     """40 experts of 16384 x 8192 codes: the last ones start past 2^31 bytes."""
     groups, n, k = 40, 16384, 8192
