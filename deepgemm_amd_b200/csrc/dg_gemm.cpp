@@ -238,8 +238,9 @@ bool cluster_allowed(const Problem& p, int cluster) {
     if (cluster == 1) return true;
     if (p.kind == DG_GEMM_M_GROUPED_RAGGED) return false;                                      // (a pair multiplies its rows with one B)
     if (p.ab_bf16 || p.reduce_batches > 1 || p.a_mn_major || p.b_mn_major) return false;       // (K-major block-scaled operands: what was measured)
-    // (measured at M = 4096; smaller GEMMs keep the one-CTA forms their cost model was fitted on)
-    return (p.kind == DG_GEMM_DENSE && p.m >= 1024) || p.kind == DG_GEMM_M_GROUPED_CONTIGUOUS;
+    // (measured at M = 4096; smaller GEMMs keep the one-CTA forms their cost model was fitted on.  A split A has twice the rows in a
+    // stage: 500 rows, N 32768 K 512, 18.1 -> 17.2 us; 768 rows, N 7168 K 2048, 24.6 -> 20.4; 256 rows, N 24576 K 1536, 20.4 -> 18.6)
+    return (p.kind == DG_GEMM_DENSE && p.m >= (p.planes == 2 ? 256 : 1024)) || p.kind == DG_GEMM_M_GROUPED_CONTIGUOUS;
 }
 
 // Layout of a candidate with the deepest pipeline that fits shared memory.  `item_kb` is the number of K-blocks (of
@@ -467,7 +468,9 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
                 if (splits > 1 && !in_cluster)   // second launch + reading S panels and writing D at a few TB/s (~2000 B per SM clock over the GPU)
                     cost += 6000.0 + static_cast<double>(splits + 1) * p.m * p.n * 4.0 / 2000.0;
                 if (in_cluster)                  // parking a tile, the cluster barrier, bn loads per thread across the cluster
-                    cost += 600.0 * splits + 20.0 * bn;     // (fitted to a sweep over sizes and widths on six decode shapes)
+                    // (fitted to a sweep over sizes and widths on six decode shapes; a split A: 128 rows, N 4096 K 7168, 20.2 us in five
+                    //  slices, 16.6 in three; 256 rows 23.9 in three, 20.4 in two)
+                    cost += (p.planes == 2 && !a_rows ? 1800.0 : 600.0) * splits + 20.0 * bn;
                 if (best.bn == 0 || cost < best.cost - 1e-9 || (std::abs(cost - best.cost) <= 1e-9 && bn > best.bn)) {
                     best.cost = cost;
                     best.bn = bn; best.bk = bk; best.cluster = cluster; best.halves = halves;

@@ -90,7 +90,7 @@ def test_the_ragged_scheduler_visits_every_tile_of_every_group_once(counts, ctas
 
 
 def test_the_many_row_configurations():
-    """A stage holds 128 rows of both planes; CTA pairs for large dense products only; K slices only inside a cluster."""
+    """A stage holds 128 rows of both planes; CTA pairs for dense products of 256 rows on only; K slices only inside a cluster."""
     for m in (40, 64, 129, 300, 1024, 4096):
         for n, k in ((2112, 7168), (24576, 1536), (256, 128), (7168, 16384)):
             for kind, groups in ((_lib.DG_GEMM_DENSE, 1), (_lib.DG_GEMM_M_GROUPED_RAGGED, 8)):
@@ -99,7 +99,7 @@ def test_the_many_row_configurations():
                 assert cfg["smem_bytes"] <= 232448 and cfg["tmem_cols"] <= 512
                 assert cfg["num_splits"] == 1 or cfg["split_in_cluster"]
                 assert cfg["a_rows"] == (64 if m <= 64 or (groups > 1 and m <= 96 * groups) else 128)
-                assert cfg["cluster_size"] == 1 or (kind == _lib.DG_GEMM_DENSE and m >= 1024)
+                assert cfg["cluster_size"] == 1 or (kind == _lib.DG_GEMM_DENSE and m >= 256)
     with pytest.raises(RuntimeError):
         dg.get_gemm_config(_lib.DG_GEMM_M_GROUPED_RAGGED, 256, 512, 512, num_groups=2, b_is_fp4=True, gran_k_b=32)
     with pytest.raises(RuntimeError):
