@@ -127,12 +127,13 @@ __device__ __forceinline__ int from_lane(int v, int l) { return __reduce_add_syn
 
 // The items in their order: groups, in a group its blocks of 128 columns, for each of them the passes of kTokens rows.  Lane l of a warp
 // holds group `window + l`, so finding an item takes a ballot, and 32 groups are passed over with one load.
+template <int tokens>
 struct Items {
-    int groups, tiles, tokens, window = -32, before = 0;      // items of the groups ahead of the window
+    int groups, tiles, window = -32, before = 0;              // items of the groups ahead of the window
     int my_first = 0, my_rows = 0, my_end = 0;                // this lane's group: its rows, the items up to and with it
     int group, first, rows, row, n0;                          // the item: its group, that one's rows, first row of the pass, first column
 
-    __device__ Items(const Bf16Fp4Params& p, int groups_, int tokens_) : groups(groups_), tiles((p.n + 127) / 128), tokens(tokens_) {
+    __device__ explicit Items(const Bf16Fp4Params& p) : groups(p.groups), tiles((p.n + 127) / 128) {
         group = first = row = 0;
         rows = p.m;
     }
@@ -169,8 +170,9 @@ struct Items {
         first = from_lane(my_first, l);
         rows = from_lane(my_rows, l);
         const int passes = (rows + tokens - 1) / tokens, local = item - (from_lane(my_end, l) - tiles * passes);
-        row = first + local % passes * tokens;
-        n0 = local / passes * 128;
+        const int tile = passes == 1 ? local : local / passes;
+        row = first + (local - tile * passes) * tokens;
+        n0 = tile * 128;
         return true;
     }
     __device__ __forceinline__ int rows_here() const { return min(tokens, first + rows - row); }
@@ -226,7 +228,7 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     const int kb0 = min(static_cast<int>(rank) * per_slice, num_blocks), kb1 = min(kb0 + per_slice, num_blocks);
     const bool some = kb1 > kb0;                 // (a slice beyond the end of K has nothing to add)
     const int step = gridDim.x / slices, first_item = blockIdx.x / slices;
-    Items at(p, p.groups, kTokens);
+    Items<kTokens> at(p);
     uint32_t stage = 0, phase = 0;
     auto advance = [&]() {
         stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -271,9 +273,16 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
             }
             fence_mbar_init();
         }
-        __syncwarp();
-        if (kSplit) griddep_wait();
-        if (at.find(p, first_item)) {
+    } else if (warp == 2) {
+        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
+        tmem_relinquish<1>();
+    }
+    __syncwarp();
+    // (every warp by itself, here: a ragged product's first item takes ~1 us to find)
+    if (kSplit) griddep_wait();
+    bool found = at.find(p, first_item);
+    if (warp == 0) {
+        if (found) {
             ahead = min(kb0 + static_cast<int>(kStages), kb1);
             for (int kb = kb0; kb < ahead; ++kb, ++stage) {
                 if (elect_one()) {
@@ -283,9 +292,6 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
             }
             stage = 0;
         }
-    } else if (warp == 2) {
-        tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_slot)), S::kTmemCols);
-        tmem_relinquish<1>();
     }
     __syncwarp();
     tc_fence_before_sync();
@@ -299,7 +305,7 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
 
     // Every warp walks the same items and K-blocks
     uint32_t count = 0, steps = 0;               // items so far: accumulator count % 2; their K-blocks (splitting warps)
-    for (int item = first_item; at.find(p, item); item += step, ++count) {
+    for (int item = first_item; found; item += step, found = at.find(p, item), ++count) {
         const uint32_t accum = count & 1, accum_phase = count >> 1 & 1;
         // first half of a split barrier: this CTA runs, and what it received for the item before has been read
         if (slices > 1) cluster_arrive_relaxed();
