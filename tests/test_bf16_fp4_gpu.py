@@ -473,6 +473,24 @@ def test_behind_a_memset_a_copy_and_a_join_of_two_streams(captured):
     check_product(d3, a0, w, added=torch.ones_like(d3))
 
 
+@pytest.mark.usefixtures("form")
+def test_the_smallest_activations():
+    """Subnormal numbers and blocks below 2^-115, where the split's scale has reached its end: an element is held to 2^-21 of its block's largest, or
+    to 2^-137 (2^-14 of the smallest scale, 2^-123)."""
+    m, n, k = 37, 136, 512
+    codes, e, w = make_weights((n, k), 32, 170, exps=(227, 236))
+    g = torch.Generator(device="cuda").manual_seed(171)
+    top = 0x80 * torch.randint(1, 14, (m, k // 32, 1), generator=g, device="cuda")               # blocks of subnormals up to blocks at 2^-114
+    bits = (torch.rand((m, k // 32, 32), generator=g, device="cuda") * top).int() + 0x8000 * torch.randint(0, 2, (m, k // 32, 32), generator=g, device="cuda")
+    a = bits.flatten(1).to(torch.int32).remainder(65536).sub(65536 * (bits.flatten(1) >= 32768)).to(torch.int16).view(torch.bfloat16)
+    d = torch.empty((m, n), dtype=torch.float, device="cuda")
+    dg.bf16_fp4_gemm_nt(a, (codes, pack_scales(e)), d)
+    x = a.double()
+    held = x.abs().unflatten(1, (k // 32, 32)).amax(-1).mul(2.0 ** -21).clamp_min(2.0 ** -137)
+    tol = (k / 8 + 64) * 2.0 ** -23 * (x.abs() @ w.abs().T) + held @ w.abs().unflatten(1, (k // 32, 32)).sum(-1).T
+    assert (x != 0).float().mean() > 0.9 and ((d.double() - x @ w.T).abs() <= tol).all()
+
+
 def test_weights_beyond_32_bit_offsets():
     """40 experts of 16384 x 8192 codes: the last ones start past 2^31 bytes."""
     groups, n, k = 40, 16384, 8192
