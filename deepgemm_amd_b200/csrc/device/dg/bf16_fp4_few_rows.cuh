@@ -198,6 +198,7 @@ template <int kTokens, bool kSplit> struct Shape {
     static_assert(kTokens <= 32, "two CTAs' shares of an SM's shared and tensor memory");
     // What a CTA receives: every slice's partial sums of the rows of D it owns
     __host__ __device__ static constexpr int recv_rows(int slices) { return (kTokens + slices - 1) / slices; }
+    static constexpr int kMostSmem = kOffRecv + (kTokens + kMaxCluster - 1) * 512;
     __host__ __device__ static constexpr int smem_bytes(int slices) { return kOffRecv + (slices > 1 ? slices * recv_rows(slices) * 512 : 0); }
 };
 

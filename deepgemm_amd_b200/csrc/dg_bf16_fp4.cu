@@ -233,7 +233,9 @@ int launch_few_rows(const dg_gemm_args_t* g, const Bf16Fp4Params& p, const Plane
     }
     const auto kernel = g->gran_k_b == 32 ? few::bf16_fp4_few_rows_kernel<kTokens, kSplit, 32> : few::bf16_fp4_few_rows_kernel<kTokens, kSplit, 128>;
     const int smem = S::smem_bytes(slices);
-    DG_CUDA_RT(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    // (the same value every time: another thread may be between these two calls)
+    static_assert(2 * (S::kMostSmem + 1024) <= 228 * 1024, "two CTAs on an SM");
+    DG_CUDA_RT(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kMostSmem));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(items, clusters_at_once(slices))) * slices);
     cfg.blockDim = dim3(S::kThreads);
