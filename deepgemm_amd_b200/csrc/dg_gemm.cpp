@@ -645,6 +645,14 @@ int encode_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uin
     }
     const Driver& drv = driver();
     if (!drv.ok) return fail(DG_ERR_CUDA, "CUDA driver unavailable: %s", drv.why.c_str());
+    // The encoder wants a current context, which a thread that has called nothing but this library does not have yet
+    CUcontext ctx = nullptr;
+    DG_CUDA_DRV(drv.cuCtxGetCurrent(&ctx));
+    if (ctx == nullptr) {
+        int device = 0;
+        DG_CUDA_RT(cudaGetDevice(&device));
+        DG_CUDA_RT(cudaSetDevice(device));
+    }
     const cuuint32_t rank = batches > 0 ? 3 : 2;
     const cuuint64_t dims[3] = {inner, outer, batches};
     const cuuint64_t strides[2] = {outer_stride_bytes, batch_stride_bytes};

@@ -491,6 +491,37 @@ def test_the_smallest_activations():
     assert (x != 0).float().mean() > 0.9 and ((d.double() - x @ w.T).abs() <= tol).all()
 
 
+def test_threads_call_at_once():
+    """Host threads with products of different forms and slices, each on a stream of its own."""
+    import threading
+    jobs = []
+    for i, (m, n, k) in enumerate([(1, 512, 4096), (6, 2112, 1024), (14, 7168, 512), (30, 1024, 2048), (90, 520, 1024), (300, 2048, 512)]):
+        codes, e, w = make_weights((n, k), 32, 180 + i)
+        jobs.append({"a": make_rows(m, k, 190 + i), "b": (codes, pack_scales(e)), "w": w, "d": torch.empty((m, n), dtype=torch.bfloat16, device="cuda"), "failed": None})
+    for j in jobs:
+        dg.bf16_fp4_gemm_nt(j["a"], j["b"], j["d"])
+        j["d"].fill_(float("nan"))
+    torch.cuda.synchronize()
+
+    def work(j):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(200):
+                    dg.bf16_fp4_gemm_nt(j["a"], j["b"], j["d"])
+                torch.cuda.current_stream().synchronize()
+        except Exception as error:          # (raised in the thread: told to the test below)
+            j["failed"] = error
+
+    threads = [threading.Thread(target=work, args=(j,)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for j in jobs:
+        assert j["failed"] is None, j["failed"]
+        check_product(j["d"], j["a"], j["w"])
+
+
 def test_weights_beyond_32_bit_offsets():
     """40 experts of 16384 x 8192 codes: the last ones start past 2^31 bytes."""
     groups, n, k = 40, 16384, 8192
