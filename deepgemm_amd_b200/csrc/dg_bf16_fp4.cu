@@ -4,8 +4,8 @@
 //     ragged   D[r, n]   =          sum over k of A[r, k] * W[g(r), n, k],   group g = rows [ends[g - 1], ends[g])
 //     W[n, k] = e2m1(code[n, k]) * 2^(scale code of (n, k / gran) - 127),    gran 32 or 128
 // The weights and their scales lie as the FP8 x FP4 GEMMs take them (codes K-major, even K in the low nibble; scales four
-// to an int32, MN-major).  An E2M1 value times a power of two times a BF16 value is exact in FP32, so the only roundings are
-// those of the FP32 sums and the one of the result.
+// to an int32, MN-major).  An E2M1 value times a power of two times a BF16 value is exact in FP32, so the roundings are those of the
+// FP32 sums, the one of the result, and what the split of A into two E4M3 vectors cannot hold (2^-21 of the largest of 32 neighbours along K).
 #include "dg_common.hpp"
 
 #include <algorithm>
