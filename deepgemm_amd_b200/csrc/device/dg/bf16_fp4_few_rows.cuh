@@ -308,8 +308,12 @@ bf16_fp4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_
     uint32_t count = 0, steps = 0;               // items so far: accumulator count % 2; their K-blocks (splitting warps)
     for (int item = first_item; found; item += step, found = at.find(p, item), ++count) {
         const uint32_t accum = count & 1, accum_phase = count >> 1 & 1;
-        // first half of a split barrier: this CTA runs, and what it received for the item before has been read
-        if (slices > 1) cluster_arrive_relaxed();
+        // first half of a split barrier: this CTA runs, and what it received for the item before has been read (so a release from the
+        // second item on: those reads come before what the peers write there next)
+        if (slices > 1) {
+            if (count == 0) cluster_arrive_relaxed();
+            else cluster_arrive();
+        }
         if (warp == 0) {
             int kb = kb0;
             if (count == 0) {
