@@ -564,7 +564,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                         }
                         sfa_slot = sfb_slot = 0;
                     }
-                    __syncwarp();
+                    if constexpr (kProducerWholeWarp) __syncwarp();
                     griddep_wait();
                     griddep_launch_dependents();
                 }
