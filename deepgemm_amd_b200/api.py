@@ -1141,8 +1141,9 @@ def bf16_fp4_gemm_nt(a, b, d, c=None, recipe_b=(1, 32), compiled_dims: str = "nk
 def m_grouped_bf16_fp4_gemm_nt_ragged(a, b, d, group_ends, recipe_b=(1, 32), compiled_dims: str = "nk") -> None:
     """D[r] = A[r] @ W[g(r)]^T for BF16 A [rows, K] sorted by expert and b = (packed E2M1 weights int8 [G, N, K/2], their
     scales): the expert layer of the 4-bit weights above.  group_ends (int32 [G], on the device, not decreasing) holds the
-    row where each group ends; the groups follow one another without padding or alignment, empty ones included, and rows
-    at or behind group_ends[-1] keep what D holds.  Capturable: a replay follows the ends of that moment.  D BF16."""
+    row where each group ends; the groups follow one another without padding or alignment, empty ones included (an end below
+    an earlier one counts as that one), and rows at or behind the last end keep what D holds.  Capturable: a replay follows
+    the ends of that moment.  D BF16."""
     if _C is not None and _C.bf16_fp4(a, b, d, None, group_ends, recipe_b, None):
         return
     w, _ = b

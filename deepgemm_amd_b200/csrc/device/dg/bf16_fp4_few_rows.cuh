@@ -49,17 +49,6 @@ struct Bf16Fp4Params {
     int groups;
 };
 
-// Rows [first, end) of group g; ends outside [0, m] or before their predecessor give an empty group rather than a wild access
-__device__ __forceinline__ void group_rows(const Bf16Fp4Params& p, int g, int& first, int& end) {
-    first = 0;
-    end = p.m;
-    if (p.group_ends != nullptr) {
-        // (from L2: with A split ahead they are read before the kernel before this one is done)
-        first = g == 0 ? 0 : min(max(__ldcg(p.group_ends + g - 1), 0), p.m);
-        end = min(max(__ldcg(p.group_ends + g), 0), p.m);
-    }
-}
-
 // One thread's share of the split: N pieces of eight elements of a row, the four threads of an aligned quad holding 32 consecutive ones.
 // hi, lo: eight E4M3 values each; code: UE8M0 code of hi's scale (lo's is 4 less), 255 (NaN) for a block with an infinity or NaN.
 template <int N>
@@ -130,6 +119,7 @@ __device__ __forceinline__ int from_lane(int v, int l) { return __reduce_add_syn
 template <int tokens>
 struct Items {
     int groups, tiles, window = -32, before = 0;              // items of the groups ahead of the window
+    int window_first = 0;                                     // where the groups ahead of the window end
     int my_first = 0, my_rows = 0, my_end = 0;                // this lane's group: its rows, the items up to and with it
     int group, first, rows, row, n0;                          // the item: its group, that one's rows, first row of the pass, first column
 
@@ -152,10 +142,25 @@ struct Items {
             window += 32;
             before = end;
             const int g = window + static_cast<int>(lane_id());
-            int last = 0;
-            my_first = 0;
-            if (g < groups) group_rows(p, g, my_first, last);
-            my_rows = max(last - my_first, 0);
+            // A group begins where the one before it ends; an end outside [0, m] is moved to its border, one before an earlier end is that one.
+            // (From L2: with A split ahead they are read before the kernel before this one is done)
+            int last = g < groups ? min(max(__ldcg(p.group_ends + g), 0), p.m) : p.m;
+            auto previous = [&]() {
+                const int v = __shfl_up_sync(0xFFFFFFFFu, last, 1);
+                return lane_id() == 0 ? window_first : v;
+            };
+            my_first = previous();
+            if (__any_sync(0xFFFFFFFFu, last < my_first)) {   // ends that go back: the largest so far
+                last = max(last, window_first);
+                #pragma unroll
+                for (int off = 1; off < 32; off *= 2) {
+                    const int v = __shfl_up_sync(0xFFFFFFFFu, last, off);
+                    if (static_cast<int>(lane_id()) >= off) last = max(last, v);
+                }
+                my_first = previous();
+            }
+            window_first = from_lane(last, 31);
+            my_rows = g < groups ? last - my_first : 0;
             my_end = tiles * ((my_rows + tokens - 1) / tokens);
             #pragma unroll
             for (int off = 1; off < 32; off *= 2) {

@@ -20,8 +20,9 @@
 //       K-blocks and the first packed scale row of the group.  layout[g] is the slice's length (a multiple
 //       of the alignment) or, in the prefix-sum form, the element where it ends, the next slice starting
 //       at the following multiple of the alignment (scheduler/gemm.cuh:226-250 of the reference).
-//   m-grouped ragged : layout[g] is the row of D where group g ends and group g + 1 starts, no padding between them; the rows of A lie in
-//       slots, the groups' first ones on multiples of four (first_slot).  Walked on the device like the masked layout.
+//   m-grouped ragged : layout[g] is the row of D where group g ends and group g + 1 starts, no padding between them (an end before
+//       an earlier one counts as that one: an empty group); the rows of A lie in slots, the groups' first ones on multiples of four
+//       (first_slot).  Walked on the device like the masked layout.
 //   batched : num_groups independent GEMMs of one shape; tile_id = batch * tiles_per_batch + tile, the
 //       batch being the third tensor-map coordinate of every operand (scheduler/gemm.cuh:251-263).
 #pragma once
@@ -205,7 +206,8 @@ struct TileScheduler {
                 const int e = layout[cur_group];
 #endif
                 uint32_t end = e < 0 ? 0u : (static_cast<uint32_t>(e) > shape_m ? shape_m : static_cast<uint32_t>(e));
-                rows = end > group_start ? end - group_start : 0u;
+                if (end < group_start) end = group_start;
+                rows = end - group_start;
                 mb = (rows + kBlockM - 1) / kBlockM;
                 if (tile_id < group_first_tile + mb * num_n_blocks) break;
                 group_first_tile += mb * num_n_blocks;

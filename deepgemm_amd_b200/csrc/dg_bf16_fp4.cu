@@ -145,8 +145,19 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const __nv_bfloat16* a,
         const int lane = threadIdx.x, mine = row0 + lane;
         int group = 0, first = 0;
         if (group_ends != nullptr) {
+            int before = 0;                                                  // the largest end of the groups ahead
             for (int g0 = 0; g0 < groups; g0 += 32) {
-                const int end = g0 + lane < groups ? min(max(__ldcg(group_ends + g0 + lane), 0), m) : INT32_MAX;
+                int end = g0 + lane < groups ? min(max(__ldcg(group_ends + g0 + lane), 0), m) : INT32_MAX;
+                const int previous = __shfl_up_sync(0xFFFFFFFFu, end, 1);
+                if (__any_sync(0xFFFFFFFFu, end < (lane == 0 ? before : previous))) {      // an end that goes back is the largest so far
+                    end = max(end, before);
+                    #pragma unroll
+                    for (int off = 1; off < 32; off *= 2) {
+                        const int v = __shfl_up_sync(0xFFFFFFFFu, end, off);
+                        if (lane >= off) end = max(end, v);
+                    }
+                }
+                before = __shfl_sync(0xFFFFFFFFu, end, 31);
                 #pragma unroll
                 for (int i = 0; i < kSplitRows; ++i) {
                     const int behind = __popc(__ballot_sync(0xFFFFFFFFu, end <= row0 + i));

@@ -226,7 +226,8 @@ DG_API int dg_fp8_bmm(const dg_gemm_args_t* args);
  * form.  k % 128 == 0; a and d 16-byte aligned rows, b 32-byte aligned rows.  accumulate, alpha: dense form only.
  * ragged: grouped_layout = int32[num_groups] on the device, the row where each group ends; group g is the rows
  * [grouped_layout[g - 1], grouped_layout[g]) (from row 0 for g = 0) of A [m, k] and D [m, n], with no padding between
- * groups and no alignment; ends must not decrease; rows at or behind the last end are not written.
+ * groups and no alignment; rows at or behind the last end are not written.  The ends do not decrease: one below an earlier
+ * end counts as that one (an empty group), one outside [0, m] as the nearer border.
  * Sums are FP32, one rounding per element of D.  The elements of A are held to 2^-21 of the largest of their 32 neighbours along K (exactly,
  * down to 2^-13 of it; not below 2^-137).  A row of A with an infinity or a NaN gives non-finite results.
  * workspace: device memory of this call alone until it has completed, 128-byte aligned, at least
