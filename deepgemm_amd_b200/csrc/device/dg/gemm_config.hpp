@@ -33,8 +33,8 @@ struct GemmLayout {
                                                    // memory and lands in accumulator rows that are never stored
 
     uint32_t planes = 1;                           // 2: A is a BF16 matrix split into two E4M3 planes; a stage holds block_m rows of each, both
-                                                   // multiplied with the stage's B into one accumulator (a_rows == 64: 64 rows of each, one above
-                                                   // the other in one MMA)
+                                                   // multiplied with the stage's B (a_rows == 64: 64 rows of each, one above the other in one MMA)
+    uint32_t plane_sums = 1;                       // accumulators of a tile: 1, or 2: one per plane
 
     // A packed scale word covers 4 * gran_k elements of K: it is fetched on every `period`-th K-block of a work item,
     // into the next of a ring of buffers.  A buffer may be refilled once the fetch it held is no longer among the
@@ -99,11 +99,13 @@ struct GemmLayout {
     }
 
     // Tensor memory: two accumulators of block_n columns (two tiles in flight when block_m is 128, the two 128-row
-    // halves of one tile when it is 256), then SFA (4 columns per 128 rows) and SFB (4 columns per 128 columns of the tile)
-    DG_HDC uint32_t tmem_col_sfa() const { return 2 * block_n; }
+    // halves of one tile when it is 256; with an accumulator per plane one tile's two, or two tiles' where four fit), then SFA
+    // (4 columns per 128 rows) and SFB (4 columns per 128 columns of the tile)
+    DG_HDC uint32_t tiles_in_flight() const { return block_m == 256 ? 1 : plane_sums == 1 || 4 * block_n + 8 + sf_block_n() / 32 <= kTmemCapacityCols ? 2 : 1; }
+    DG_HDC uint32_t tmem_col_sfa() const { return block_m == 256 ? 2 * block_n : tiles_in_flight() * plane_sums * block_n; }
     // (per packed word of a stage: kind::mxf4 stages hold two)
     DG_HDC uint32_t tmem_col_sfb() const { return tmem_col_sfa() + block_m / 32 * sfa_words() * planes; }
-    DG_HDC uint32_t tmem_cols_used() const { return ab_elem_bytes != 1 ? 2 * block_n : tmem_col_sfb() + sf_block_n() / 32 * sfb_words(); }
+    DG_HDC uint32_t tmem_cols_used() const { return ab_elem_bytes != 1 ? tmem_col_sfa() : tmem_col_sfb() + sf_block_n() / 32 * sfb_words(); }
     DG_HDC uint32_t tmem_cols_alloc() const {
         const uint32_t u = tmem_cols_used();
         return u <= 32 ? 32 : u <= 64 ? 64 : u <= 128 ? 128 : u <= 256 ? 256 : 512;

@@ -44,7 +44,10 @@
 // the rearranging warp's work and the scale columns of tensor memory disappear; MN-major atoms are 64 elements wide.
 //
 // DG_PLANES == 2: A is a BF16 matrix split into two E4M3 matrices, A = hi + lo with a scale per 32 elements of K each (dg_bf16_fp4.cu), and
-// the product is hi B^T + lo B^T: a stage holds 128 rows of either and one B, which both MMAs of a K-block read into one accumulator.  Two
+// the product is hi B^T + lo B^T: a stage holds 128 rows of either and one B, which both MMAs of a K-block read.  DG_PLANE_SUMS is 2 where K is
+// long: the planes have an accumulator each, added in the epilogue.  The tensor cores cut off what an FP32 accumulator cannot hold instead of rounding it;
+// hi's products, of six significant bits under power-of-two scales, leave next to nothing to cut off, lo's a 16th of it, but in one accumulator
+// every step with lo cuts (K 16384: off by 7.3e-6 of the root mean square, 5.9e-6 of it toward zero; a chain of rounded FP32 sums 9e-7).  Two
 // E4M3 x E2M1 MMAs take the time of one in BF16, without B ever being widened.  A tile of which at most 64 rows count ("half": a small group, or
 // the end of one) is one MMA instead of two: hi's 64 rows above lo's in one 128-row operand, added up in the epilogue.
 //
@@ -161,8 +164,10 @@ constexpr uint32_t CTA_M = BLOCK_M * kMHalves;             // rows of A (and D) 
 constexpr uint32_t TILE_M = kAllHalf ? 64 : CTA_M * kCluster;        // rows of D per scheduled tile
 // Four role warps and one epilogue warpgroup per 128 rows of the CTA's tile
 constexpr uint32_t kNumThreads = 128 + 128 * kMHalves, kNumEpilogueThreads = 128, kEpilogueWarpBase = 4;
-// Tensor memory holds two accumulators: two tiles in flight, or the two halves of one
-constexpr uint32_t kNumAccumStages = kMHalves == 1 ? 2 : 1;
+#ifndef DG_PLANE_SUMS
+#define DG_PLANE_SUMS 1
+#endif
+constexpr uint32_t kSums = DG_PLANE_SUMS;                  // accumulators of a tile (split A: one for both planes, or one each)
 
 static_assert(BLOCK_N % 16 == 0 && BLOCK_N >= 16 && BLOCK_N <= (kHasSF ? 240 : 256), "UMMA_N must be a multiple of 16 that leaves room for the scales");
 static_assert(!kABIsBF16 || (!kAIsFP4 && !kBIsFP4 && BLOCK_K == 128), "BF16 operands: 128-byte stages");
@@ -237,12 +242,15 @@ static_assert(kSplitCluster == 1 || (kGemmType == kDense && !kSplitK && kCluster
 #define DG_EPILOGUE_BACKOFF_NS 0
 #endif
 constexpr GemmLayout kLayout{CTA_M, BLOCK_N, BLOCK_K, kNumStages, kDElemBytes, kCluster, kBMnMajor ? 1u : 0u, kGranKA, kGranKB,
-                             DG_SHORT_K, kABElemBytes, DG_STORE_BUFFERS, kMXF4 ? 1u : 0u, DG_A_ROWS, kPlanes};
+                             DG_SHORT_K, kABElemBytes, DG_STORE_BUFFERS, kMXF4 ? 1u : 0u, DG_A_ROWS, kPlanes, kSums};
+// Tensor memory holds two accumulators: two tiles in flight, or the two halves of one, or its two planes' sums (or all four)
+constexpr uint32_t kNumAccumStages = kLayout.tiles_in_flight();
 static_assert(DG_A_ROWS == 0 || (DG_A_ROWS % 8 == 0 && DG_A_ROWS < 128 && (kGemmType == kDense || kAllHalf) && kCluster == 1 && kMHalves == 1 && !kAMnMajor),
               "a shortened A stage: dense GEMMs with fewer rows than one tile (or a split A in tiles of 64), K-major A, one CTA per tile");
 static_assert(kPlanes == 1 || (kPlanes == 2 && kMHalves == 1 && kHasSF && !kMXF4 && !kAIsFP4 && !kAMnMajor && !kBMnMajor && BLOCK_K == 128 && kGranKA == 32 &&
                                (DG_A_ROWS == 0 || kAllHalf) && !kTransposedD && (kGemmType == kDense || kGemmType == kMGroupedRagged)),
               "split A: K-major E4M3 planes with one scale per 32 elements, 128 rows per CTA, dense and ragged");
+static_assert(kSums == 1 || (kSums == 2 && kPlanes == 2 && !kAllHalf), "an accumulator per plane: tiles whose planes do not share one MMA");
 static_assert(kGemmType != kMGroupedRagged || (kPlanes == 2 && kCluster == 1), "ragged groups: built for a split A, one CTA per tile");
 constexpr uint32_t kSFAWords = kHasSF ? kLayout.sfa_words() : 1, kSFBWords = kHasSF ? kLayout.sfb_words() : 1;   // packed words per row and stage
 // K coordinate of a K-major load advances by this much per K-block: elements of the tensor map's type (bytes for the
@@ -761,7 +769,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                             if (num_passes == 2 && h != pass) continue;
                             // Half h: rows [128 h, 128 h + 128) of the A stage (128 * BLOCK_K bytes further, in either layout),
                             // its own accumulator and its own four columns of row scales
-                            const uint32_t tmem_d = tmem_base + (accum + h) * UMMA_N;
+                            const uint32_t tmem_d = tmem_base + (accum * kSums + h + (kSums == 2 ? pl : 0u)) * UMMA_N;
                             #pragma unroll
                             for (uint32_t j = 0; j < BLOCK_K / UMMA_K; ++j) {
                                 // Which byte of the packed scale word applies to these 32 elements of K
@@ -780,7 +788,7 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                                 else
                                     tc_mma_mxf8f6f4<kCluster>(tmem_d, a_desc + (h + pl) * ((BLOCK_M * BLOCK_K) >> 4) + a_step(j), b_desc + b_step(j),
                                                               instr_desc_with_sf_ids(idesc, sfa_id, sfb_id),
-                                                              tmem_base + kTmemColSFA + (h + pl) * 4, tmem_base + kTmemColSFB, ((kb - kb0) | j | pl) != 0);
+                                                              tmem_base + kTmemColSFA + (h + pl) * 4, tmem_base + kTmemColSFB, ((kb - kb0) | j | (kSums == 2 ? 0u : pl)) != 0);
                             }
                         }
                         DG_PROF_FINE_ADD(prof_mma, prof_i1);
@@ -900,11 +908,18 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
         // With BF16 output a thread therefore first moves its whole accumulator row into registers (packed, BLOCK_N / 2
         // of them) and hands tensor memory back before any staging or store.  Otherwise (a spare accumulator, or FP32
         // output, whose rows would need twice the registers) the row is read group by group.
-        constexpr bool kRowInRegs = kMHalves == 2 && !kDIsFP32;
+        // (Two planes' sums that leave room for one tile are the same case)
+        constexpr bool kRowInRegs = (kMHalves == 2 || (kSums == 2 && kNumAccumStages == 1)) && !kDIsFP32;
         constexpr uint32_t kGroupBytes = kLayout.group_bytes();
         bool ok = true;
         [[maybe_unused]] uint32_t cluster_barriers_done = 0;
         uint32_t tile_iter = 0, store_iter = 0;
+        // An accumulator per plane: the other one's columns are loaded beside the first one's and added to them (a half tile has both planes in the
+        // first, one below the other)
+        auto add_plane = [&](uint32_t (&v)[16], const uint32_t (&w)[16]) {
+            #pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(w[i]));
+        };
         DG_PROF_VAR(prof_wait); DG_PROF_VAR(prof_store);
         DG_PROF_BEGIN(prof_t0);
         while (ok && sched.next(tile)) {
@@ -962,8 +977,13 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                 #pragma unroll
                 for (uint32_t b = 0; b < BLOCK_N / 16; ++b) {
                     uint32_t v[16];
-                    tmem_ld_32x32b_x16(tmem_base + ((quarter * 32) << 16) + accum * UMMA_N + b * 16, v);
+                    [[maybe_unused]] uint32_t w[16];
+                    const uint32_t from = tmem_base + ((quarter * 32) << 16) + accum * kSums * UMMA_N + b * 16;
+                    const bool both = kSums == 2 && !is_half(tile);
+                    tmem_ld_32x32b_x16(from, v);
+                    if (both) tmem_ld_32x32b_x16(from + UMMA_N, w);
                     tmem_ld_wait();
+                    if (both) add_plane(v, w);
                     #pragma unroll
                     for (uint32_t i = 0; i < 16; ++i) {
                         const uint32_t chunk = (b * 16 + i) / 8, owned_col = chunk / kSplitCluster * 8 + i % 8;
@@ -1083,7 +1103,8 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
             const uint32_t n0 = tile.n_block * BLOCK_N;
             const uint32_t d_row0 = tile.d_row_base + tile.m_block * TILE_M + cta_rank * CTA_M + wg * BLOCK_M +
                                     (kSplitK ? tile.split * p.split_panel_rows : 0u);
-            const uint32_t tmem_row_addr = tmem_base + ((quarter * 32) << 16) + accum * UMMA_N;
+            const uint32_t tmem_row_addr = tmem_base + ((quarter * 32) << 16) + accum * kSums * UMMA_N;
+            const bool both = kSums == 2 && !is_half(tile);
             // Rows of this 128-row part that may be written
             const uint32_t rows_before = cta_rank * CTA_M + wg * BLOCK_M;
             const uint32_t valid_rows = tile.valid_rows <= rows_before ? 0u :
@@ -1138,18 +1159,51 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                 continue;
             }
 
+            // A half tile: lanes 64 .. 127 hold lo's products of rows 0 .. 63.  Through a staging buffer (column by column, so that a warp's
+            // rows are neighbours) to the lanes that hold hi's
+            auto join_half = [&](auto& v, uint32_t cols) {
+                if constexpr (kHalfTiles) {
+                    constexpr uint32_t kLoads = sizeof(v) / sizeof(v[0]);
+                    static_assert(kLoads * 16 * 64 * 4 <= kStoreStageBytes, "64 rows in FP32 fit a staging buffer");
+                    if (!is_half(tile)) return;
+                    if (epi_tid == 0) tma_store_wait_read<0>();
+                    named_barrier_sync(bar_id, kNumEpilogueThreads);
+                    if (row_in_tile >= 64) {
+                        #pragma unroll
+                        for (uint32_t c = 0; c < kLoads * 16; ++c)
+                            if (c < cols) st_shared_u32(staging + (c * 64 + row_in_tile - 64) * 4, v[c / 16][c % 16]);
+                    }
+                    named_barrier_sync(bar_id, kNumEpilogueThreads);
+                    if (row_in_tile < 64) {
+                        #pragma unroll
+                        for (uint32_t c = 0; c < kLoads * 16; ++c)
+                            if (c < cols) v[c / 16][c % 16] = __float_as_uint(__uint_as_float(v[c / 16][c % 16]) +
+                                                                              __uint_as_float(ld_shared_u32(staging + (c * 64 + row_in_tile) * 4)));
+                    }
+                    named_barrier_sync(bar_id, kNumEpilogueThreads);
+                }
+            };
+
             [[maybe_unused]] uint32_t row[kRowInRegs ? BLOCK_N / 2 : 1];        // BF16 pairs: columns (2i, 2i+1) of the tile row
             if constexpr (kRowInRegs) {
                 // 32 columns per round trip to tensor memory (more in flight cost registers the row itself needs:
                 // 48 and 64 columns spilled and measured 3-20 % slower)
-                constexpr uint32_t kLoadsPerTrip = 2;
+                constexpr uint32_t kLoadsPerTrip = kSums == 2 && !kHalfTiles ? 1 : 2;
                 #pragma unroll
                 for (uint32_t b = 0; b < BLOCK_N / 16; b += kLoadsPerTrip) {
                     uint32_t v[kLoadsPerTrip][16];
+                    [[maybe_unused]] uint32_t w[kLoadsPerTrip][16];
                     #pragma unroll
                     for (uint32_t l = 0; l < kLoadsPerTrip; ++l)
-                        if (b + l < BLOCK_N / 16) tmem_ld_32x32b_x16(tmem_row_addr + (b + l) * 16, v[l]);
+                        if (b + l < BLOCK_N / 16) {
+                            tmem_ld_32x32b_x16(tmem_row_addr + (b + l) * 16, v[l]);
+                            if (both) tmem_ld_32x32b_x16(tmem_row_addr + UMMA_N + (b + l) * 16, w[l]);
+                        }
                     tmem_ld_wait();
+                    #pragma unroll
+                    for (uint32_t l = 0; l < kLoadsPerTrip; ++l)
+                        if (both && b + l < BLOCK_N / 16) add_plane(v[l], w[l]);
+                    join_half(v, BLOCK_N - b * 16 < kLoadsPerTrip * 16 ? BLOCK_N - b * 16 : kLoadsPerTrip * 16);
                     #pragma unroll
                     for (uint32_t l = 0; l < kLoadsPerTrip; ++l)
                         if (b + l < BLOCK_N / 16) {
@@ -1176,11 +1230,19 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                 constexpr uint32_t kMaxLoads = (kGroupCols + 15) / 16;
                 [[maybe_unused]] uint32_t v[kRowInRegs ? 1 : kMaxLoads][16];
                 if constexpr (!kRowInRegs) {
+                    [[maybe_unused]] uint32_t w[kMaxLoads][16];
                     #pragma unroll
                     for (uint32_t l = 0; l < kMaxLoads; ++l)
-                        if (l * 16 < kCols) tmem_ld_32x32b_x16(tmem_row_addr + g * kGroupCols + l * 16, v[l]);
+                        if (l * 16 < kCols) {
+                            tmem_ld_32x32b_x16(tmem_row_addr + g * kGroupCols + l * 16, v[l]);
+                            if (both) tmem_ld_32x32b_x16(tmem_row_addr + UMMA_N + g * kGroupCols + l * 16, w[l]);
+                        }
                     tmem_ld_wait();
                     if (g + 1 == kNumGroups) release_tmem();           // the last of the accumulator is in registers
+                    #pragma unroll
+                    for (uint32_t l = 0; l < kMaxLoads; ++l)
+                        if (both && l * 16 < kCols) add_plane(v[l], w[l]);
+                    join_half(v, kCols);
                     #pragma unroll
                     for (uint32_t l = 0; l < kMaxLoads; ++l)
                         if (l * 16 < kCols) {
@@ -1188,27 +1250,6 @@ dg_gemm_fp8_fp4(const __grid_constant__ CUtensorMap tm_a,
                             for (uint32_t i = 0; i < 16; ++i)
                                 v[l][i] = __float_as_uint(__uint_as_float(v[l][i]) * p.alpha);
                         }
-                }
-                if constexpr (kHalfTiles) {
-                    if (is_half(tile)) {
-                        // Lanes 64 .. 127 hold lo's products of rows 0 .. 63: through a staging buffer (column by column, so that a warp's
-                        // rows are neighbours) to the lanes that hold hi's
-                        if (epi_tid == 0) tma_store_wait_read<0>();
-                        named_barrier_sync(bar_id, kNumEpilogueThreads);
-                        if (row_in_tile >= 64) {
-                            #pragma unroll
-                            for (uint32_t c = 0; c < kGroupCols; ++c)
-                                if (c < kCols) st_shared_u32(staging + (c * 64 + row_in_tile - 64) * 4, v[c / 16][c % 16]);
-                        }
-                        named_barrier_sync(bar_id, kNumEpilogueThreads);
-                        if (row_in_tile < 64) {
-                            #pragma unroll
-                            for (uint32_t c = 0; c < kGroupCols; ++c)
-                                if (c < kCols) v[c / 16][c % 16] = __float_as_uint(__uint_as_float(v[c / 16][c % 16]) +
-                                                                                   __uint_as_float(ld_shared_u32(staging + (c * 64 + row_in_tile) * 4)));
-                        }
-                        named_barrier_sync(bar_id, kNumEpilogueThreads);
-                    }
                 }
                 // Quantised output: the group's BF16-rounded values, 32 columns per scale, as e4m3 words; the scale bytes
                 // go straight to global memory (one byte per row and 32 columns)

@@ -257,6 +257,14 @@ GemmLayout fit_stages(GemmLayout lay, int64_t item_kb, int max_stages) {
     return best;
 }
 
+// Accumulators of a tile of a split A whose planes take an MMA each.  In one accumulator every step with lo cuts off what FP32 cannot hold: off by
+// 2.1e-7 (root mean square, of the sums') at K 512, 8.1e-7 at 2048, 2.7e-6 at 7168, 7.3e-6 at 16384; with one each 1.8e-7 at 2048, 6.3e-7, 1.7e-6; FP32
+// sums rounded one by one 1.1e-7, 2.6e-7, 5.3e-7, 9.3e-7.  Wide tiles then leave no spare accumulator for the next one: 4096 rows, N 7168 K 2048, 98.4 -> 103 us; 500
+// rows, N 32768 K 512, 20.0 -> 22.9; 8191 rows in 32 groups, N 4096 K 7168, 535 -> 538.  A BF16 D rounds to 2^-9, so it takes one up to K 2048, an FP32 D up to 512.
+uint32_t plane_sums(const Problem& p, int64_t item_k, int a_rows) {
+    return p.planes == 2 && a_rows == 0 && item_k > (p.d_fp32 ? 512 : 2048) ? 2 : 1;
+}
+
 // How many thread-block clusters of S CTAs (one CTA per SM) run at once.  A cluster lives inside one GPC, so the answer
 // is the sum over GPCs of floor(SMs of the GPC / S), which only the driver knows: the table holds what it reported for
 // kernels launched so far (cuOccupancyMaxActiveClusters), and until then the numbers of one B200, scaled by the SM count.
@@ -413,7 +421,8 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
                 GemmLayout lay{128u * halves, static_cast<uint32_t>(bn), static_cast<uint32_t>(bk), 2,
                                static_cast<uint32_t>(splits > 1 && !in_cluster ? 4 : d_elem), static_cast<uint32_t>(cluster),
                                p.b_mn_major ? 1u : 0u, static_cast<uint32_t>(p.gran_k_a), static_cast<uint32_t>(p.gran_k_b), 0u,
-                               static_cast<uint32_t>(ab_elem), store_buffers, p.mxf4 ? 1u : 0u, static_cast<uint32_t>(a_rows), static_cast<uint32_t>(p.planes)};
+                               static_cast<uint32_t>(ab_elem), store_buffers, p.mxf4 ? 1u : 0u, static_cast<uint32_t>(a_rows), static_cast<uint32_t>(p.planes),
+                               plane_sums(p, item_k, a_rows)};
                 const GemmLayout unfitted = lay;
                 lay = fit_stages(lay, p.kind == DG_GEMM_K_GROUPED_CONTIGUOUS ? 0 : item_kb, max_stages);   // slices may be one K-block
                 if (lay.num_stages <= 2 && env_int("FORCE_STORE_BUFFERS") != 2) {
@@ -464,7 +473,9 @@ int choose_config_for(const Problem& p, dg_gemm_config_t* cfg, const Constraints
                 double cost = static_cast<double>(waves) * std::max(per_tile, epilogue) + epilogue + 2000.0;
                 // 256-row tiles have no spare accumulator: the next tile's MMAs start once the epilogue warpgroups have
                 // moved their rows from tensor memory into registers (~1400 cycles, measured)
-                if (halves == 2) cost = static_cast<double>(waves) * (per_tile + 1400.0) + epilogue + 2000.0;
+                // (two planes' sums in FP32 are read as they are stored, the whole epilogue)
+                if (lay.tiles_in_flight() == 1)
+                    cost = static_cast<double>(waves) * (per_tile + (lay.plane_sums == 2 && p.d_fp32 ? epilogue : 1400.0)) + epilogue + 2000.0;
                 if (splits > 1 && !in_cluster)   // second launch + reading S panels and writing D at a few TB/s (~2000 B per SM clock over the GPU)
                     cost += 6000.0 + static_cast<double>(splits + 1) * p.m * p.n * 4.0 / 2000.0;
                 if (in_cluster)                  // parking a tile, the cluster barrier, bn loads per thread across the cluster
@@ -571,7 +582,8 @@ GemmLayout layout_of(const Problem& p, const dg_gemm_config_t& cfg) {
                    static_cast<uint32_t>(cfg.cluster_size), p.b_mn_major ? 1u : 0u,
                    static_cast<uint32_t>(p.gran_k_a), static_cast<uint32_t>(p.gran_k_b),
                    item_kb < cfg.num_stages ? 1u : 0u, static_cast<uint32_t>(ab_elem), static_cast<uint32_t>(cfg.store_buffers),
-                   p.mxf4 ? 1u : 0u, cfg.a_rows > 0 && cfg.a_rows < cfg.block_m ? static_cast<uint32_t>(cfg.a_rows) : 0u, static_cast<uint32_t>(p.planes)};
+                   p.mxf4 ? 1u : 0u, cfg.a_rows > 0 && cfg.a_rows < cfg.block_m ? static_cast<uint32_t>(cfg.a_rows) : 0u, static_cast<uint32_t>(p.planes),
+                   plane_sums(p, std::min<int64_t>(p.k, static_cast<int64_t>(cfg.kb_per_split) * 128), cfg.a_rows < cfg.block_m ? cfg.a_rows : 0)};
     return lay;
 }
 
@@ -612,6 +624,7 @@ std::string generate_source(const Problem& p, const dg_gemm_config_t& cfg) {
       << "#define DG_PRODUCER_WHOLE_WARP " << env_int("PRODUCER_WHOLE_WARP", 1) << "\n"
       << "#define DG_L2_HINT " << env_int("L2_HINT", 0) << "\n"
       << "#define DG_PLANES " << p.planes << "\n"
+      << "#define DG_PLANE_SUMS " << layout_of(p, cfg).plane_sums << "\n"
       << "#include <dg/gemm_fp8_fp4.cuh>\n";
     return s.str();
 }

@@ -23,3 +23,77 @@ def test_clusters_that_take_several_items(m, n, k):
         first = d
     check_product(first, a, w)
     assert dg.kernel_status() == 0
+
+
+def exact_planes(m, n, k, step, seed):
+    """Rows and weights of one sign whose products FP32 can add up without rounding, plane by plane, but not both planes in one sum.
+
+    Blocks of 32 elements of K are in turn [1, 1.75] and 2^-step times that: x / s is in [256, 448] with s = 2^-8 (or 2^-(8 + step)), so hi is a multiple of 32 and
+    16 times the rest, a multiple of 32 of at most 256, is lo, exactly.  Weights are 0.5 .. 6 with the scale 1.  The products of hi are multiples of
+    2^-(4 + step), those of lo of 2^-(8 + step)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = 1 + torch.randint(0, 97, (m, k), generator=g, device="cuda") / 128.0
+    x *= torch.where(torch.arange(k, device="cuda") // 32 % 2 == 0, 1.0, 2.0 ** -step)
+    codes = torch.randint(1, 8, (n, k // 2, 2), generator=g, device="cuda", dtype=torch.int32)
+    w = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device="cuda", dtype=torch.float64)[codes.flatten(1)]
+    packed = (codes[..., 0] | codes[..., 1] << 4).to(torch.int8)
+    # the premise: hi's sum is below 2^24 of its steps, and so is lo's with all of its parts (|rest| <= 2^-4) of one sign
+    hi_sum, lo_sum = (x.double() + 2.0 ** -4) @ w.T, torch.where(x >= 1, 2.0 ** -4, 2.0 ** (-4 - step)).double() @ w.T
+    assert hi_sum.max() < 2.0 ** (24 - 4 - step) and lo_sum.max() < 2.0 ** (24 - 8 - step)
+    return x.to(torch.bfloat16), packed, torch.full((n, k // 32), 127, dtype=torch.uint8, device="cuda"), w
+
+
+@pytest.mark.usefixtures("form")
+@pytest.mark.parametrize("m,n,k,step,accumulate", [(1, 264, 2048, 6, False), (24, 264, 7168, 3, False), (64, 264, 7168, 3, True), (200, 264, 7168, 3, True), (200, 264, 16384, 2, True),
+                                                   (1500, 1032, 7168, 3, False), (2100, 1032, 16384, 2, False), (300, 520, 2048, 6, False), (700, 520, 2048, 6, True)])
+def test_sums_that_fp32_holds_are_not_cut_off(m, n, k, step, accumulate):
+    """What FP32 holds of a plane's sum has to come out of it.  The roundings left are those of adding the planes (one for each slice of K, at most
+    eight) and the slices (one each): 2^-24 of the result for each of 16.  (Accumulating onto zeros: one slice only, in the GEMM form.)"""
+    a, codes, e, w = exact_planes(m, n, k, step, 230)
+    d = torch.zeros((m, n), dtype=torch.float, device="cuda")
+    dg.bf16_fp4_gemm_nt(a, (codes, pack_scales(e)), d, c=d if accumulate else None)
+    want = a.double() @ w.T
+    assert ((d.double() - want).abs() <= 16 * 2.0 ** -24 * want).all(), ((d.double() - want) / want).abs().max().item() * 2.0 ** 24
+
+
+def check_rounded(d, a, w):
+    want = a.double() @ w.T
+    half_step = torch.exp2(torch.floor(torch.log2(want)) - 8)
+    assert ((d.double() - want).abs() <= half_step + 16 * 2.0 ** -24 * want).all()
+
+
+@pytest.mark.usefixtures("form")
+@pytest.mark.parametrize("m,n,k,step", [(24, 264, 7168, 3), (700, 520, 7168, 3), (2100, 1032, 16384, 2), (2100, 1032, 7168, 3)])
+def test_bf16_results_are_those_sums_rounded(m, n, k, step):
+    """The same sums, off by half a BF16 step and those 16 roundings: one that was cut off is on the wrong side of a border now and then."""
+    a, codes, e, w = exact_planes(m, n, k, step, 231)
+    d = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    dg.bf16_fp4_gemm_nt(a, (codes, pack_scales(e)), d)
+    check_rounded(d, a, w)
+
+
+@pytest.mark.usefixtures("form")
+@pytest.mark.parametrize("counts,k,step", [([9, 0, 30, 1], 7168, 3), ([300, 64, 1, 129], 7168, 3), ([700, 0, 450], 16384, 2)])
+def test_ragged_results_are_those_sums_rounded(counts, k, step):
+    n, ends = 520, torch.tensor(counts, device="cuda").cumsum(0).to(torch.int32)
+    parts = [exact_planes(max(c, 1), n, k, step, 232 + i) for i, c in enumerate(counts)]
+    a = torch.cat([p[0][:c] for p, c in zip(parts, counts)])
+    d = torch.empty((a.size(0), n), dtype=torch.bfloat16, device="cuda")
+    dg.m_grouped_bf16_fp4_gemm_nt_ragged(a, (torch.stack([p[1] for p in parts]), pack_scales(torch.stack([p[2] for p in parts]))), d, ends)
+    for i, (p, c) in enumerate(zip(parts, counts)):
+        if c:
+            check_rounded(d[int(ends[i]) - c:int(ends[i])], p[0], p[3])
+
+
+@pytest.mark.usefixtures("form")
+@pytest.mark.parametrize("m,n,k", [(16, 520, 7168), (64, 520, 16384), (300, 520, 512), (300, 520, 1024), (600, 1032, 2048), (2100, 1032, 7168), (2100, 1032, 16384)])
+def test_errors_are_those_of_a_chain_of_rounded_sums(m, n, k):
+    """Against K products added in FP32 one after the other: every addition is off by at most half a step of a partial sum, 2^-24 of it, independently, and the
+    partial sums of K independent terms are sqrt(i / K) of the last one, so the errors' root mean square is at most 2^-24 sqrt(K / 2) of the sums'."""
+    codes, e, w = make_weights((n, k), 32, 240)
+    a = make_rows(m, k, 241)
+    d = torch.empty((m, n), dtype=torch.float, device="cuda")
+    dg.bf16_fp4_gemm_nt(a, (codes, pack_scales(e)), d)
+    want = a.double() @ w.T
+    ratio = ((d.double() - want).pow(2).mean() / want.pow(2).mean()).sqrt().item()
+    assert ratio <= 2.0 ** -24 * (k / 2) ** 0.5, ratio * 2.0 ** 24
