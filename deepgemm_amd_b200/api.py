@@ -1110,7 +1110,7 @@ def bf16_fp4_gemm_nt(a, b, d, c=None, recipe_b=(1, 32), compiled_dims: str = "nk
     """D[M,N] = C + alpha * A[M,K] @ W[N,K]^T for BF16 A and b = (packed E2M1 weights int8 [N, K/2], their scales): the
     weights an FP8 x FP4 GEMM takes, in the same storage, multiplied with activations that are not quantised.  recipe_b =
     (1, 32) or (1, 128); scales packed (int32) or FP32 (packed on the fly); D BF16 or FP32; K % 128 == 0.  Any number of
-    rows from a single token on; sums in FP32, one rounding per element (two where C is added to a BF16 D); the elements of A
+    rows from a single token on; sums in FP32, one rounding per element (two where many rows are added to a BF16 C); the elements of A
     are held to 2^-21 of the largest of their 32 neighbours along K."""
     if _C is not None and _C.bf16_fp4(a, b, d, c, None, recipe_b, alpha):
         return

@@ -6,6 +6,8 @@
 // The weights and their scales lie as the FP8 x FP4 GEMMs take them (codes K-major, even K in the low nibble; scales four
 // to an int32, MN-major).  An E2M1 value times a power of two times a BF16 value is exact in FP32, so the roundings are those of the
 // FP32 sums, the one of the result, and what the split of A into two E4M3 vectors cannot hold (2^-21 of the largest of 32 neighbours along K).
+// A BF16 D that is added to is rounded once by the few-row kernel, which adds in FP32, and twice by the GEMM, whose TMA copy adds the rounded product: reading D in
+// its epilogue instead took 500 rows, N 32768 K 512, from 29.5 us to 37.7 and 4096 rows, N 7168 K 2048, from 87 to 93.
 #include "dg_common.hpp"
 
 #include <algorithm>

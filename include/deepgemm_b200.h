@@ -228,7 +228,8 @@ DG_API int dg_fp8_bmm(const dg_gemm_args_t* args);
  * [grouped_layout[g - 1], grouped_layout[g]) (from row 0 for g = 0) of A [m, k] and D [m, n], with no padding between
  * groups and no alignment; rows at or behind the last end are not written.  The ends do not decrease: one below an earlier
  * end counts as that one (an empty group), one outside [0, m] as the nearer border.
- * Sums are FP32, one rounding per element of D.  The elements of A are held to 2^-21 of the largest of their 32 neighbours along K (exactly,
+ * Sums are FP32, one rounding per element of D; where many rows accumulate into a BF16 D, two: alpha A W^T to BF16, then its sum
+ * with D (few rows: one, of the FP32 sum with D).  The elements of A are held to 2^-21 of the largest of their 32 neighbours along K (exactly,
  * down to 2^-13 of it; not below 2^-137).  A row of A with an infinity or a NaN gives non-finite results.
  * workspace: device memory of this call alone until it has completed, 128-byte aligned, at least
  * dg_bf16_fp4_workspace_bytes(args, ragged) bytes (0 for a few rows or weights, about 2 m k above; it reads only the

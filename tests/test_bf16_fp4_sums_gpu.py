@@ -97,3 +97,27 @@ def test_errors_are_those_of_a_chain_of_rounded_sums(m, n, k):
     want = a.double() @ w.T
     ratio = ((d.double() - want).pow(2).mean() / want.pow(2).mean()).sqrt().item()
     assert ratio <= 2.0 ** -24 * (k / 2) ** 0.5, ratio * 2.0 ** 24
+
+
+@pytest.mark.parametrize("few", [1, 2, 3, 4])
+@pytest.mark.parametrize("m,n,k", [(5, 392, 640), (30, 264, 1024), (64, 331, 640), (190, 264, 2304)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_few_rows_meet_a_bf16_c_in_fp32(m, n, k, in_place, few, monkeypatch):
+    """C nearly cancels the product, and the one rounding is of their sum.  With S = sum |a| |w|: chains of at most K / 8 + 64 additions off by
+    2^-23 S each, as for every product; the planes hold A to 2^-21 of a block's largest element; alpha and C, one FP32 rounding each of
+    at most 2^-23 S; the result's, 2^-8 of it."""
+    monkeypatch.setenv("DG_FORCE_BF16_FP4_FORM", str(few))
+    codes, e, w = make_weights((n, k), 32, 250)
+    a, alpha = make_rows(m, k, 251), -0.37
+    exact = float(torch.tensor(alpha)) * (a.double() @ w.T)
+    c = (exact * -(1 + 2.0 ** -6 * torch.rand(exact.shape, generator=torch.Generator(device="cuda").manual_seed(252), device="cuda"))).to(torch.bfloat16)
+    wide = torch.full((m, (n + 7) // 8 * 8), float("nan"), dtype=torch.bfloat16, device="cuda")
+    d = wide[:, :n]
+    if in_place:
+        d.copy_(c)
+    dg.bf16_fp4_gemm_nt(a, (codes, pack_scales(e)), d, c=d if in_place else c, alpha=alpha)
+    want, s = exact + c.double(), abs(alpha) * (a.double().abs() @ w.abs().T)
+    held = abs(alpha) * 2.0 ** -21 * (a.double().abs().unflatten(1, (k // 32, 32)).amax(-1) @ w.abs().unflatten(1, (k // 32, 32)).sum(-1).T)
+    tol = ((k / 8 + 66) * 2.0 ** -23 * s + held) * (1 + 2.0 ** -7) + 2.0 ** -8 * want.abs() * (1 + 2.0 ** -7)
+    off = (d.double() - want).abs()
+    assert (off <= tol).all(), (off / tol).max().item()
