@@ -1050,6 +1050,24 @@ int dg_gemm_precompile(int kind, const dg_gemm_args_t* args) {
     return get_kernel(p, cfg, &kernel);
 }
 
+int dg_enumerate_ragged_tiles(int block_m, int block_n, int raster_group, int shape_m, int shape_n, int num_groups,
+                              const int32_t* ends_host, int cta, int num_ctas, uint32_t* out, int max_tiles) {
+    if (!((block_m == 64 || block_m == 128) && block_n > 0 && raster_group > 0 && num_ctas > 0 && cta >= 0 && cta < num_ctas && shape_m >= 0 && shape_n >= 0 &&
+          num_groups >= 0 && (num_groups == 0 || ends_host != nullptr))) {
+        fail(DG_ERR_INVALID_ARGUMENT, "Assertion error (%s:%d): bad scheduler arguments", __FILE__, __LINE__);
+        return -DG_ERR_INVALID_ARGUMENT;
+    }
+    TileScheduler<kMGroupedRagged> sched(block_m, block_n, raster_group, shape_m, shape_n, num_groups, ends_host, cta, num_ctas);
+    int count = 0;
+    for (Tile t; sched.next(t); ++count) {
+        if (count >= max_tiles || out == nullptr) continue;
+        const uint32_t first = t.m_block * static_cast<uint32_t>(block_m);
+        const uint32_t words[5] = {t.d_row_base + first, t.n_block, t.group, t.valid_rows, t.a_row_base + first};
+        std::copy(words, words + 5, out + 5 * count);
+    }
+    return count;
+}
+
 int dg_enumerate_tiles(int kind, int block_n, int raster_group, int shape_m, int shape_n, int num_groups,
                        const int32_t* layout_host, int cta, int num_ctas, uint32_t* out, int max_tiles) {
     if (!(block_n > 0 && raster_group > 0 && num_ctas > 0 && cta >= 0 && cta < num_ctas && shape_m >= 0 && shape_n >= 0)) {

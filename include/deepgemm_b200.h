@@ -294,6 +294,10 @@ DG_API int dg_get_gemm_config(int kind, const dg_gemm_args_t* args, dg_gemm_conf
  * max_tiles are written) or a negative dg_status_t. */
 DG_API int dg_enumerate_tiles(int kind, int block_n, int raster_group, int shape_m, int shape_n, int num_groups,
                        const int32_t* layout_host, int cta, int num_ctas, uint32_t* out, int max_tiles);
+/* The ragged layout's walk in tiles of block_m (64 or 128) rows, five uint32 per tile {first row of D, n_block, group, valid_rows, first
+ * row of the split A}: the rows of A lie in slots, every group's from a multiple of four on. */
+DG_API int dg_enumerate_ragged_tiles(int block_m, int block_n, int raster_group, int shape_m, int shape_n, int num_groups,
+                       const int32_t* ends_host, int cta, int num_ctas, uint32_t* out, int max_tiles);
 
 /* ---- JIT runtime: csrc/runtime/jit.hpp + third-party/deep_jit (README.md:164-191) --------------- */
 
