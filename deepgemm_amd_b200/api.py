@@ -1108,10 +1108,12 @@ def _on_device_of(t: torch.Tensor):
 
 def bf16_fp4_gemm_nt(a, b, d, c=None, recipe_b=(1, 32), compiled_dims: str = "nk", alpha: Optional[float] = None) -> None:
     """D[M,N] = C + alpha * A[M,K] @ W[N,K]^T for BF16 A and b = (packed E2M1 weights int8 [N, K/2], their scales): the
-    weights an FP8 x FP4 GEMM takes, in the same storage, multiplied with activations that are not quantised.  recipe_b =
-    (1, 32) or (1, 128); scales packed (int32) or FP32 (packed on the fly); D BF16 or FP32; K % 128 == 0.  Any number of
-    rows from a single token on; sums in FP32, one rounding per element (two where many rows are added to a BF16 C); the elements of A
-    are held to 2^-21 of the largest of their 32 neighbours along K."""
+    weights an FP8 x FP4 GEMM takes, in the same storage, multiplied with activations in BF16.  recipe_b = (1, 32) or
+    (1, 128); scales packed (int32) or FP32 (packed on the fly); D BF16 or FP32; K % 128 == 0.  Any number of rows from a
+    single token on; sums in FP32, one rounding per element (two where many rows are added to a BF16 C).  The elements of A
+    are held to 2^-21 of the largest of their 32 neighbours along K: exactly down to 2^-13 of it, with fewer bits below.  A
+    row with an infinity or a NaN gives NaN.  More than some 32 rows want rows of D of whole 16-byte pieces (N a multiple of
+    8 in BF16, 4 in FP32): other N read the weights once for every 32 rows."""
     if _C is not None and _C.bf16_fp4(a, b, d, c, None, recipe_b, alpha):
         return
     w, _ = b
@@ -1143,7 +1145,7 @@ def m_grouped_bf16_fp4_gemm_nt_ragged(a, b, d, group_ends, recipe_b=(1, 32), com
     scales): the expert layer of the 4-bit weights above.  group_ends (int32 [G], on the device, not decreasing) holds the
     row where each group ends; the groups follow one another without padding or alignment, empty ones included (an end below
     an earlier one counts as that one), and rows at or behind the last end keep what D holds.  Capturable: a replay follows
-    the ends of that moment.  D BF16."""
+    the ends of that moment.  D BF16.  A is held, and N is best a multiple of 8, as above."""
     if _C is not None and _C.bf16_fp4(a, b, d, None, group_ends, recipe_b, None):
         return
     w, _ = b

@@ -30,7 +30,9 @@ int clusters_at_once(int slices) {
 
 // The few-row kernel's variants, and what a launch of each takes: so many us, and so many more for each K-block (128 x 128 weights) that a CTA
 // goes through, alone on its SM or next to another one.  Fitted to 265 launches of dense products of 1 to 64 rows, N x K from 512 x 4096 to
-// 7168 x 16384, in one to eight slices (4 to 95 us): half of them are met within 5 %, nine of ten within 13 %.  Splitting A costs a CTA
+// 7168 x 16384, in one to eight slices (4 to 95 us): half of them are met within 5 %, nine of ten within 13 %.  Ragged products, which read the
+// ends before their first load, take it as it is: 8 rows in 32 groups of N 4096 K 7168 24.9 us for 25.4 measured, 131 rows of N 7168 K 2048 42.7 for 41.2, but
+// 37 rows in 4 groups of N 2112 K 1536 6.4 for 8.5.  Splitting A costs a CTA
 // instructions for every block (1 row 0.33 us, 8 rows 0.37); A split ahead costs a kernel more (0.8 us outside of a graph, half of it counted).
 struct FewRows {
     int tokens;

@@ -260,7 +260,8 @@ GemmLayout fit_stages(GemmLayout lay, int64_t item_kb, int max_stages) {
 // Accumulators of a tile of a split A whose planes take an MMA each.  In one accumulator every step with lo cuts off what FP32 cannot hold: off by
 // 2.1e-7 (root mean square, of the sums') at K 512, 8.1e-7 at 2048, 2.7e-6 at 7168, 7.3e-6 at 16384; with one each 1.8e-7 at 2048, 6.3e-7, 1.7e-6; FP32
 // sums rounded one by one 1.1e-7, 2.6e-7, 5.3e-7, 9.3e-7.  Wide tiles then leave no spare accumulator for the next one: 4096 rows, N 7168 K 2048, 98.4 -> 103 us; 500
-// rows, N 32768 K 512, 20.0 -> 22.9; 8191 rows in 32 groups, N 4096 K 7168, 535 -> 538.  A BF16 D rounds to 2^-9, so it takes one up to K 2048, an FP32 D up to 512.
+// rows, N 32768 K 512, 20.0 -> 22.9; 8191 rows in 32 groups, N 4096 K 7168, 535 -> 538; FP32 D: 500 rows, N 32768 K 1024, 34.8 -> 38.9, 4096 rows, N 7168 K 2048, 88 -> 94,
+// 2048 rows, N 4096 K 7168, 94 both.  A BF16 D rounds to 2^-9 of its own, so it takes one accumulator up to K 2048, an FP32 D up to 512.
 uint32_t plane_sums(const Problem& p, int64_t item_k, int a_rows) {
     return p.planes == 2 && a_rows == 0 && item_k > (p.d_fp32 ? 512 : 2048) ? 2 : 1;
 }

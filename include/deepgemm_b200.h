@@ -230,7 +230,8 @@ DG_API int dg_fp8_bmm(const dg_gemm_args_t* args);
  * end counts as that one (an empty group), one outside [0, m] as the nearer border.
  * Sums are FP32, one rounding per element of D; where many rows accumulate into a BF16 D, two: alpha A W^T to BF16, then its sum
  * with D (few rows: one, of the FP32 sum with D).  The elements of A are held to 2^-21 of the largest of their 32 neighbours along K (exactly,
- * down to 2^-13 of it; not below 2^-137).  A row of A with an infinity or a NaN gives non-finite results.
+ * down to 2^-13 of it; not below 2^-137).  A row of A with an infinity or a NaN gives NaN, sums within a 16th of FP32's largest number may
+ * come out infinite.  More than some 32 rows of D that are not whole 16-byte pieces (n * element size) read the weights once for every 32.
  * workspace: device memory of this call alone until it has completed, 128-byte aligned, at least
  * dg_bf16_fp4_workspace_bytes(args, ragged) bytes (0 for a few rows or weights, about 2 m k above; it reads only the
  * sizes, num_groups and d_dtype in args; -1: no valid sizes). */
