@@ -8,15 +8,15 @@ from test_bf16_fp4_gpu import check_product, check_ragged, make_rows, make_weigh
 pytestmark = pytest.mark.gpu
 
 SETTINGS = [{"PRODUCER_WHOLE_WARP": "0"}, {"MMA_WHOLE_WARP": "0"}, {"PRODUCER_WHOLE_WARP": "0", "MMA_WHOLE_WARP": "0"}, {"L2_HINT": "1"}, {"L2_HINT": "2"},
-            {"EPILOGUE_BACKOFF_NS": "100"}, {"FORCE_STORE_BUFFERS": "2"}]
+            {"EPILOGUE_BACKOFF_NS": "100"}, {"FORCE_STORE_BUFFERS": "2"}, {"PROFILE": "1"}]
 
 
 @pytest.mark.parametrize("settings", SETTINGS, ids=lambda s: "-".join(f"{k}={v}" for k, v in s.items()))
 def test_the_gemm_form_gives_the_same_bits(settings, monkeypatch):
-    """Tiles of 64 rows, whole tiles, CTA pairs, K slices in a cluster; dense and ragged, twice in a row (the second launch behind the first)."""
+    """Tiles of 64 rows, whole tiles, CTA pairs, K slices in a cluster, a sum per plane; dense and ragged, twice in a row (the second launch behind the first)."""
     monkeypatch.setenv("DG_FORCE_BF16_FP4_FORM", "5")
     jobs = []
-    for m, n, k in ((40, 264, 2048), (150, 520, 640), (600, 1032, 768)):
+    for m, n, k in ((40, 264, 2048), (150, 520, 640), (600, 1032, 768), (1100, 2056, 2304)):
         codes, e, w = make_weights((n, k), 32, 210)
         jobs.append((make_rows(m, k, 211), (codes, pack_scales(e)), w, torch.empty((m, n), dtype=torch.bfloat16, device="cuda")))
     grouped = [(counts, ragged_case(counts, 2, 264, 640, 32, 212)) for counts in ([40, 0, 61, 3], [300, 64, 0, 129])]

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import deepgemm_amd_b200 as dg
-from test_bf16_fp4_gpu import check_product, form, make_rows, make_weights, pack_scales  # noqa: F401  (form: a fixture)
+from test_bf16_fp4_gpu import check_product, check_ragged, form, make_rows, make_weights, pack_scales, ragged_case  # noqa: F401  (form: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +121,34 @@ def test_few_rows_meet_a_bf16_c_in_fp32(m, n, k, in_place, few, monkeypatch):
     tol = ((k / 8 + 66) * 2.0 ** -23 * s + held) * (1 + 2.0 ** -7) + 2.0 ** -8 * want.abs() * (1 + 2.0 ** -7)
     off = (d.double() - want).abs()
     assert (off <= tol).all(), (off / tol).max().item()
+
+
+@pytest.mark.parametrize("m,n,k,out", [(700, 4104, 2304, torch.bfloat16), (2300, 7176, 2304, torch.bfloat16), (200, 8200, 2304, torch.bfloat16), (700, 4104, 1152, torch.float),
+                                       (200, 8204, 1152, torch.float), (3000, 2056, 640, torch.float)])
+@pytest.mark.parametrize("alpha,accumulate", [(None, False), (-0.5, False), (2.0, True)])
+@pytest.mark.parametrize("block_n", [0, 112, 128, 240])
+def test_tiles_with_a_sum_per_plane(m, n, k, out, alpha, accumulate, block_n, monkeypatch):
+    """Widths that leave tensor memory room for two tiles' sums (up to 112 columns) and for one tile's; one CTA and pairs; the last tile of 64 rows or fewer."""
+    monkeypatch.setenv("DG_FORCE_BF16_FP4_FORM", "5")
+    if block_n:
+        monkeypatch.setenv("DG_FORCE_BLOCK_N", str(block_n))
+    codes, e, w = make_weights((n, k), 32, 280)
+    a, c = make_rows(m, k, 281), torch.randn((m, n), device="cuda").to(out)
+    d = torch.full((m, n + 8), -7.0, dtype=out, device="cuda")[:, :n]
+    dg.bf16_fp4_gemm_nt(a, (codes, pack_scales(e)), d, c=c if accumulate else None, alpha=alpha)
+    check_product(d, a, w, added=c if accumulate else None, alpha=1.0 if alpha is None else alpha)
+    assert dg.kernel_status() == 0
+
+
+@pytest.mark.parametrize("block_n", [0, 112, 240])
+@pytest.mark.parametrize("counts", [[300, 129, 64, 700, 0, 1], [128, 192, 20, 513], [2000, 63, 65]])
+def test_ragged_tiles_with_a_sum_per_plane(counts, block_n, monkeypatch):
+    monkeypatch.setenv("DG_FORCE_BF16_FP4_FORM", "5")
+    if block_n:
+        monkeypatch.setenv("DG_FORCE_BLOCK_N", str(block_n))
+    n, k = 4104, 2304
+    codes, e, w, a, ends = ragged_case(counts, 2, n, k, 32, 282)
+    d = torch.full((a.size(0), n), -7.0, dtype=torch.bfloat16, device="cuda")
+    dg.m_grouped_bf16_fp4_gemm_nt_ragged(a, (codes, pack_scales(e)), d, ends)
+    check_ragged(d, a, w, counts, -7.0)
+    assert dg.kernel_status() == 0
