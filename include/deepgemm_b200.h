@@ -228,7 +228,8 @@ DG_API int dg_fp8_bmm(const dg_gemm_args_t* args);
  * [grouped_layout[g - 1], grouped_layout[g]) (from row 0 for g = 0) of A [m, k] and D [m, n], with no padding between
  * groups and no alignment; rows at or behind the last end are not written.  The ends do not decrease: one below an earlier
  * end counts as that one (an empty group), one outside [0, m] as the nearer border.
- * Sums are FP32, one rounding per element of D; where many rows accumulate into a BF16 D, two: alpha A W^T to BF16, then its sum
+ * Sums are the tensor cores' FP32, which cut off where they cannot hold a bit (off by 1e-7 to 2e-6, K 512 to 16384, of the results' root mean
+ * square); one rounding per element of D; where many rows accumulate into a BF16 D, two: alpha A W^T to BF16, then its sum
  * with D (few rows: one, of the FP32 sum with D).  The elements of A are held to 2^-21 of the largest of their 32 neighbours along K (exactly,
  * down to 2^-13 of it; not below 2^-137).  A row of A with an infinity or a NaN gives NaN, sums within a 16th of FP32's largest number may
  * come out infinite.  More than some 32 rows of D that are not whole 16-byte pieces (n * element size) read the weights once for every 32.
